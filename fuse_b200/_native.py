@@ -273,12 +273,47 @@ class Mxfp8OprojBackwardParams(_Record):
                 ("weight_mode", C.c_int32)]
 
 
+class RmsNormParams(C.Structure):
+    _fields_ = [("input", C.c_void_p), ("residual", C.c_void_p), ("gamma", C.c_void_p),
+                ("residual_output", C.c_void_p), ("output", C.c_void_p), ("quantized", Mxfp8Activation),
+                ("input_stride", C.c_int64), ("residual_stride", C.c_int64), ("residual_output_stride", C.c_int64),
+                ("output_stride", C.c_int64), ("rows", C.c_int64), ("hidden", C.c_int32), ("epsilon", C.c_float)]
+
+
+class RmsNormBackwardParams(C.Structure):
+    _fields_ = [("grad_output", C.c_void_p), ("stream_input", C.c_void_p), ("gamma", C.c_void_p),
+                ("grad_stream", C.c_void_p), ("grad_input", C.c_void_p), ("grad_gamma", C.c_void_p),
+                ("grad_output_stride", C.c_int64), ("stream_input_stride", C.c_int64),
+                ("grad_stream_stride", C.c_int64), ("grad_input_stride", C.c_int64), ("rows", C.c_int64),
+                ("hidden", C.c_int32), ("epsilon", C.c_float), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "wavelength": 3, "yarn": 4}
+
+
+class RotarySpec(C.Structure):
+    _fields_ = [("theta", C.c_double), ("factor", C.c_double), ("low_freq_factor", C.c_double),
+                ("high_freq_factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("magnitude", C.c_double), ("original_context", C.c_int64), ("rotary_dim", C.c_int32),
+                ("scaling", C.c_int32), ("interleaved", C.c_uint8)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_output", C.c_void_p), ("k_output", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("q_output_stride", C.c_int64),
+                ("k_output_stride", C.c_int64), ("positions", C.c_void_p), ("position_start", C.c_int64),
+                ("rows", C.c_int64), ("seq_len", C.c_int64), ("spec", RotarySpec), ("q_heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("position_bytes", C.c_int32),
+                ("adjoint", C.c_uint8)]
+
+
 ABI_RECORDS = {0: GemmProblem, 1: UlyssesRoute, 2: GemmA2AParams, 3: A2AGemmParams,
                4: KernelTraits, 5: Options, 17: Mxfp8QkvBackwardDataParams, 18: Mxfp8QkvBackwardWeightParams,
                19: Mxfp8QkvBackwardParams, 20: Mxfp8OprojBackwardDataParams, 21: Mxfp8OprojBackwardWeightParams,
                22: Mxfp8OprojBackwardParams, 15: GroupedGemmPolicy, 16: Bf16GroupedGemmParams, 14: Mxfp8A2AGemmParams, 12: Mxfp8Activation, 13: Mxfp8GemmA2AParams, 6: QkvBackwardDataParams, 7: QkvBackwardWeightParams,
                8: QkvBackwardParams, 9: OprojBackwardDataParams, 10: OprojBackwardWeightParams,
-               11: OprojBackwardParams}
+               11: OprojBackwardParams, 23: RmsNormParams, 24: RmsNormBackwardParams, 25: RotarySpec, 26: RotaryParams}
 
 # Every symbol include/fuse_b200.h declares: name -> (restype, argtypes).
 _P = C.c_void_p
@@ -348,6 +383,11 @@ SYMBOLS = {
                                  C.POINTER(C.c_double * 5)]),
     "fuse_b200_plan_remote": (C.c_int, [C.c_int32, C.c_double, C.c_double, C.c_int64, C.c_int32, C.c_int32, C.c_int32,
                                         C.c_int32, C.c_double, C.POINTER(C.c_double * 5)]),
+    "fuse_b200_launch_rms_norm": (C.c_int, [C.POINTER(RmsNormParams), _P]),
+    "fuse_b200_rms_norm_backward_workspace_size": (C.c_int, [C.c_int64, C.c_int32, C.POINTER(C.c_size_t)]),
+    "fuse_b200_launch_rms_norm_backward": (C.c_int, [C.POINTER(RmsNormBackwardParams), _P]),
+    "fuse_b200_rotary_frequencies": (C.c_int, [C.POINTER(RotarySpec), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "fuse_b200_launch_rotary": (C.c_int, [C.POINTER(RotaryParams), _P]),
     "fuse_b200_generate_bf16": (C.c_int, [_P, C.c_uint64, C.c_uint64, C.c_float, C.c_int, _P]),
     "fuse_b200_tile_order_decode": (C.c_int, [C.c_int32] * 4 + [C.c_int64, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "fuse_b200_select_swizzle": (C.c_int32, [C.c_int32] * 3),

@@ -339,3 +339,33 @@ def launch_gemm_a2a_mxfp8_static(params: Mxfp8GemmA2AParams, stream: int = 0) ->
     """MXFP8 QKV operator with the library's built-in weight scratch (allocates nothing;
     weights whose scratch exceeds N.STATIC_SCRATCH_BYTES are rejected)."""
     return N.lib().fuse_b200_launch_gemm_a2a_mxfp8_static(C.byref(params), stream)
+
+
+# ---- block operators: residual RMS norm, rotary positions (include/fuse_b200.h) ------------------
+from ._native import RmsNormBackwardParams, RmsNormParams, RotaryParams, RotarySpec  # noqa: E402,F401
+
+
+def launch_rms_norm(params: RmsNormParams, stream: int = 0) -> int:
+    """h = input + residual; y = h / rms(h) * gamma, as BF16 and / or MXFP8."""
+    return N.lib().fuse_b200_launch_rms_norm(C.byref(params), stream)
+
+
+def rms_norm_backward_workspace_size(rows: int, hidden: int):
+    size = C.c_size_t()
+    rc = N.lib().fuse_b200_rms_norm_backward_workspace_size(rows, hidden, C.byref(size))
+    return rc, size.value
+
+
+def launch_rms_norm_backward(params: RmsNormBackwardParams, stream: int = 0) -> int:
+    return N.lib().fuse_b200_launch_rms_norm_backward(C.byref(params), stream)
+
+
+def rotary_frequencies(spec: RotarySpec):
+    """(cudaError, radians per position of every pair, magnitude) -- host only."""
+    out, magnitude = (C.c_double * max(1, spec.rotary_dim // 2))(), C.c_double()
+    rc = N.lib().fuse_b200_rotary_frequencies(C.byref(spec), out, C.byref(magnitude))
+    return rc, list(out) if rc == 0 else [], magnitude.value
+
+
+def launch_rotary(params: RotaryParams, stream: int = 0) -> int:
+    return N.lib().fuse_b200_launch_rotary(C.byref(params), stream)

@@ -1,0 +1,288 @@
+"""The operators of a transformer block between and before the fused projections, on torch tensors.
+
+    y, h = rms_norm(x, gamma, residual=h)                 # -> proj.qkv(y, w_qkv)
+    h, data, scales = rms_norm_mxfp8(x, gamma, h)         # -> the MXFP8 QKV projection's prequantised activation
+    q, k = rotary(q, k, Rotary(128), head_dim=128)        # on the planar Q and K the all-to-all leaves
+
+Tensors are BF16 [rows, width] on one CUDA device, rows `width` apart or more (views of wider tensors
+do, with row strides of a multiple of 8 elements); a tensor that an operator cannot take is refused, never copied.
+Work runs on the tensors' device and on its current stream.  Gradients come through torch.autograd
+where an argument requires them.  The C entry points underneath are in include/fuse_b200.h."""
+from __future__ import annotations
+
+import ctypes as C
+import dataclasses
+
+import torch
+
+from . import _native as N
+
+BF16 = torch.bfloat16
+
+
+def _check(rc: int, what: str) -> None:
+    if rc != 0:
+        raise RuntimeError(f"{what} -> cudaError {rc}")
+
+
+def _rows(t: torch.Tensor, name: str, width: int | None = None, rows: int | None = None, device=None) -> None:
+    if (not isinstance(t, torch.Tensor) or t.dtype != BF16 or t.dim() != 2 or not t.is_cuda or
+            (t.shape[1] != 1 and t.stride(1) != 1) or (width is not None and t.shape[1] != width) or
+            (rows is not None and t.shape[0] != rows) or (device is not None and t.device != device)):
+        raise ValueError(f"{name}: expected a bfloat16 CUDA tensor [{'rows' if rows is None else rows}, "
+                         f"{'width' if width is None else width}] with contiguous rows"
+                         f"{'' if device is None else f' on {device}'}, got "
+                         f"{(t.dtype, tuple(t.shape), t.stride(), t.device) if isinstance(t, torch.Tensor) else type(t)}")
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else -1
+
+
+def _grad(g: torch.Tensor) -> torch.Tensor:
+    """A gradient as autograd hands it over (it may be expanded, transposed or unaligned) as rows an operator takes."""
+    if g.stride(1) == 1 and g.data_ptr() % 16 == 0 and (g.shape[0] == 1 or (g.stride(0) >= g.shape[1] and g.stride(0) % 8 == 0)):
+        return g
+    return g.clone(memory_format=torch.contiguous_format)
+
+
+class _On:
+    """Makes a tensor's device the current one for a launch, where it is not already."""
+    __slots__ = ("index", "back")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------------------------------------ RMS norm
+def _norm_arguments(x, gamma, residual):
+    _rows(x, "x")
+    if residual is not None:
+        _rows(residual, "residual", x.shape[1], x.shape[0], x.device)
+    if gamma.dtype != BF16 or tuple(gamma.shape) != (x.shape[1],) or not gamma.is_contiguous() or gamma.device != x.device:
+        raise ValueError(f"gamma: expected contiguous bfloat16 ({x.shape[1]},) on {x.device}, got {gamma.dtype} "
+                         f"{tuple(gamma.shape)} on {gamma.device}")
+
+
+def _norm_forward(x, gamma, residual, eps, output: bool, mxfp8: bool):
+    rows, hidden = x.shape
+    p = N.RmsNormParams()
+    p.input, p.gamma, p.rows, p.hidden, p.epsilon = x.data_ptr(), gamma.data_ptr(), rows, hidden, eps
+    p.input_stride = _stride(x)
+    p.residual_output_stride = p.output_stride = -1
+    h, y, data, scales = x, None, None, None
+    if residual is not None:
+        h = torch.empty((rows, hidden), dtype=BF16, device=x.device)
+        p.residual, p.residual_stride, p.residual_output = residual.data_ptr(), _stride(residual), h.data_ptr()
+    if output:
+        y = torch.empty((rows, hidden), dtype=BF16, device=x.device)
+        p.output = y.data_ptr()
+    if mxfp8:
+        if hidden % 32:
+            raise ValueError(f"an MXFP8 output needs rows of a multiple of 32 elements, got {hidden}")
+        data = torch.empty((rows, hidden), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(N.lib().fuse_b200_mxfp8_scale_bytes(rows, hidden), dtype=torch.uint8, device=x.device)
+        p.quantized.data, p.quantized.scales = data.data_ptr(), scales.data_ptr()
+        p.quantized.data_bytes, p.quantized.scale_bytes = data.numel(), scales.numel()
+    if rows:
+        with _On(x) as stream:
+            _check(N.lib().fuse_b200_launch_rms_norm(C.byref(p), stream), "launch_rms_norm")
+    return y, h, data, scales
+
+
+def _norm_backward(dy, dh, h, gamma, eps, want_gamma: bool):
+    rows, hidden = h.shape
+    p = N.RmsNormBackwardParams()
+    dy = _grad(dy)
+    dx = torch.empty((rows, hidden), dtype=BF16, device=h.device)
+    p.grad_output, p.grad_output_stride = dy.data_ptr(), _stride(dy)
+    p.stream_input, p.stream_input_stride = h.data_ptr(), _stride(h)
+    if dh is not None:
+        dh = _grad(dh)
+        p.grad_stream, p.grad_stream_stride = dh.data_ptr(), _stride(dh)
+    p.gamma, p.grad_input, p.grad_input_stride = gamma.data_ptr(), dx.data_ptr(), -1
+    p.rows, p.hidden, p.epsilon = rows, hidden, eps
+    dgamma = None
+    with _On(h) as stream:
+        if want_gamma:
+            size = C.c_size_t()
+            _check(N.lib().fuse_b200_rms_norm_backward_workspace_size(rows, hidden, C.byref(size)),
+                   "rms_norm_backward_workspace_size")
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=h.device)
+            dgamma = torch.empty(hidden, dtype=BF16, device=h.device)
+            p.grad_gamma, p.workspace, p.workspace_bytes = dgamma.data_ptr(), workspace.data_ptr(), size.value
+        _check(N.lib().fuse_b200_launch_rms_norm_backward(C.byref(p), stream), "launch_rms_norm_backward")
+    return dx, dgamma
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, residual, eps, mxfp8):
+        y, h, data, scales = _norm_forward(x, gamma, residual, eps, True, mxfp8)
+        ctx.save_for_backward(h, gamma)
+        ctx.eps, ctx.summed = eps, residual is not None
+        ctx.set_materialize_grads(False)
+        if mxfp8:
+            ctx.mark_non_differentiable(data, scales)
+        return y, h if residual is not None else None, data, scales
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh, _data, _scales):
+        h, gamma = ctx.saved_tensors
+        if dy is None:
+            return dh, None, dh if ctx.summed else None, None, None
+        dx, dgamma = _norm_backward(dy, dh, h, gamma, ctx.eps, ctx.needs_input_grad[1])
+        return dx, dgamma, dx if ctx.summed else None, None, None
+
+
+def rms_norm(x: torch.Tensor, gamma: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6,
+             mxfp8: bool = False):
+    """h = x + residual (BF16, or x itself without a residual); y = h / sqrt(mean(h^2) + eps) * gamma.
+    Returns (y, h), with `mxfp8` (y, h, data, scales): the E4M3 bytes [rows, hidden] of y and its UE8M0 scales in
+    native atoms, what the MXFP8 projections take.  hidden: a multiple of 8 (32 with mxfp8), at most 16384."""
+    _norm_arguments(x, gamma, residual)
+    if _wants_grad(x, gamma, residual):
+        y, h, data, scales = _RmsNorm.apply(x, gamma, residual, eps, mxfp8)
+        h = x if residual is None else h
+    else:
+        y, h, data, scales = _norm_forward(x, gamma, residual, eps, True, mxfp8)
+    return (y, h, data, scales) if mxfp8 else (y, h)
+
+
+def rms_norm_mxfp8(x: torch.Tensor, gamma: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
+    """The same with the MXFP8 form alone, for a forward pass that keeps no BF16 activation: (h, data, scales).
+    It has no gradient; a training step takes rms_norm(..., mxfp8=True)."""
+    _norm_arguments(x, gamma, residual)
+    if _wants_grad(x, gamma, residual):
+        raise RuntimeError("rms_norm_mxfp8 has no gradient: use rms_norm(..., mxfp8=True), or torch.no_grad()")
+    _, h, data, scales = _norm_forward(x, gamma, residual, eps, False, True)
+    return h, data, scales
+
+
+# ------------------------------------------------------------------------------------------------ rotary positions
+@dataclasses.dataclass(frozen=True)
+class Rotary:
+    """What turns: the first `rotary_dim` elements of every head, pairs (i, i + rotary_dim / 2) or, interleaved,
+    (2i, 2i + 1), at theta^(-2i / rotary_dim) radians per position, scaled for contexts longer than
+    `original_context` by "linear", "ntk", "wavelength" or "yarn" (include/fuse_b200.h has the formulas).
+    `magnitude` multiplies cosine and sine (default: 1, or yarn's 0.1 ln(factor) + 1)."""
+    rotary_dim: int
+    theta: float = 10000.0
+    interleaved: bool = False
+    scaling: str = "none"
+    factor: float = 1.0
+    original_context: int = 0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    magnitude: float = 0.0
+
+    def record(self) -> N.RotarySpec:
+        if self.scaling not in N.ROTARY_SCALINGS:
+            raise ValueError(f"scaling: one of {sorted(N.ROTARY_SCALINGS)}, got {self.scaling!r}")
+        return N.RotarySpec(self.theta, self.factor, self.low_freq_factor, self.high_freq_factor, self.beta_fast,
+                            self.beta_slow, self.magnitude, self.original_context, self.rotary_dim,
+                            N.ROTARY_SCALINGS[self.scaling], 1 if self.interleaved else 0)
+
+    def frequencies(self) -> tuple[list[float], float]:
+        """Radians per position of every pair, and the magnitude."""
+        from . import api
+        rc, values, magnitude = api.rotary_frequencies(self.record())
+        if rc != 0:
+            raise ValueError(f"not a rotary specification: {self}")
+        return values, magnitude
+
+
+def _rotary_launch(q, k, qo, ko, spec, head_dim, seq_len, start, positions, adjoint):
+    p = N.RotaryParams()
+    if q is not None:
+        p.q, p.q_output, p.q_heads = q.data_ptr(), qo.data_ptr(), q.shape[1] // head_dim
+        p.q_stride, p.q_output_stride = _stride(q), _stride(qo)
+    if k is not None:
+        p.k, p.k_output, p.kv_heads = k.data_ptr(), ko.data_ptr(), k.shape[1] // head_dim
+        p.k_stride, p.k_output_stride = _stride(k), _stride(ko)
+    if positions is not None:
+        p.positions, p.position_bytes = positions.data_ptr(), positions.element_size()
+    some = q if q is not None else k
+    p.position_start, p.rows, p.seq_len = start, some.shape[0], seq_len
+    p.head_dim, p.spec, p.adjoint = head_dim, spec, adjoint
+    with _On(some) as stream:
+        _check(N.lib().fuse_b200_launch_rotary(C.byref(p), stream), "launch_rotary")
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, spec, head_dim, seq_len, start, positions):
+        ctx.rest = (spec, head_dim, seq_len, start)
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        qo, ko = (None if t is None else torch.empty(t.shape, dtype=BF16, device=t.device) for t in (q, k))
+        _rotary_launch(q, k, qo, ko, spec, head_dim, seq_len, start, positions, 0)
+        return qo, ko
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        positions, = ctx.saved_tensors
+        dq, dk = (None if g is None else _grad(g) for g in (dq, dk))
+        if dq is None and dk is None:
+            return (None,) * 7
+        oq, ok = (None if g is None else torch.empty(g.shape, dtype=BF16, device=g.device) for g in (dq, dk))
+        spec, head_dim, seq_len, start = ctx.rest
+        _rotary_launch(dq, dk, oq, ok, spec, head_dim, seq_len, start, positions, 1)
+        return oq, ok, None, None, None, None, None
+
+
+def _rotary_arguments(q, k, spec, head_dim, seq_len, positions):
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("rotary needs q or k")
+    for t, name in ((q, "q"), (k, "k")):
+        if t is not None:
+            _rows(t, name, rows=some.shape[0], device=some.device)
+            if head_dim <= 0 or t.shape[1] % head_dim:
+                raise ValueError(f"{name}: rows of {t.shape[1]} elements are not whole heads of {head_dim}")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous() or
+                                  tuple(positions.shape) != (some.shape[0],) or positions.device != some.device):
+        raise ValueError(f"positions: expected contiguous int32 or int64 ({some.shape[0]},) on {some.device}")
+    if seq_len is None:
+        seq_len = max(1, some.shape[0])
+    return spec.record(), seq_len
+
+
+def rotary(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head_dim: int, seq_len: int | None = None,
+           start: int = 0, positions: torch.Tensor | None = None):
+    """Turned copies of q [rows, q_heads * head_dim] and k [rows, kv_heads * head_dim] (either may be None).  Row r is
+    at position positions[r], or start + r % seq_len (seq_len: all rows, one sequence)."""
+    record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, positions)
+    if _wants_grad(q, k):
+        return _Rotary.apply(q, k, record, head_dim, seq_len, start, positions)
+    qo, ko = (None if t is None else torch.empty(t.shape, dtype=BF16, device=t.device) for t in (q, k))
+    _rotary_launch(q, k, qo, ko, record, head_dim, seq_len, start, positions, 0)
+    return qo, ko
+
+
+def rotary_(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head_dim: int, seq_len: int | None = None,
+            start: int = 0, positions: torch.Tensor | None = None):
+    """The same in place (no gradient)."""
+    record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, positions)
+    if _wants_grad(q, k):
+        raise RuntimeError("rotary_ writes its arguments and has no gradient: use rotary")
+    _rotary_launch(q, k, q, k, record, head_dim, seq_len, start, positions, 0)
+    return q, k

@@ -438,6 +438,10 @@ int fuse_b200_abi_sizeof(int record) {
     case 20: return int(sizeof(fuse_mxfp8_oproj_backward_data_params));
     case 21: return int(sizeof(fuse_mxfp8_oproj_backward_weight_params));
     case 22: return int(sizeof(fuse_mxfp8_oproj_backward_params));
+    case 23: return int(sizeof(fuse_b200_rms_norm_params));
+    case 24: return int(sizeof(fuse_b200_rms_norm_backward_params));
+    case 25: return int(sizeof(fuse_b200_rotary_spec));
+    case 26: return int(sizeof(fuse_b200_rotary_params));
     default: return -1;
   }
 }

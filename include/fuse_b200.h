@@ -550,6 +550,106 @@ FUSE_API int fuse_launch_oproj_backward_mxfp8_data_ex(const fuse_mxfp8_oproj_bac
 FUSE_API int fuse_launch_oproj_backward_mxfp8_weight(const fuse_mxfp8_oproj_backward_weight_params* params, fuse_stream stream);
 FUSE_API int fuse_launch_oproj_backward_mxfp8(const fuse_mxfp8_oproj_backward_params* params, fuse_stream stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The operators of a block between and before the projections.  No entry point of the reference
+ * computes them on its own (attention_postprocess.h:13-60 names rotary positions and the residual
+ * RMS norm as epilogue stages).  BF16 tensors are [rows, width] with a row stride in elements
+ * (negative = packed); nothing is allocated; rows that an operator does not own are left as they were.
+ * ------------------------------------------------------------------------------------------- */
+
+/* h = bf16(input + residual);  y = h * rsqrt(mean(h^2) + epsilon) * gamma, the mean in FP32.
+ * hidden: a multiple of 8 (of 32 with `quantized`), at most 16384; epsilon at least 1e-30.  Strides:
+ * multiples of 8, pointers 16-byte aligned.  `residual` may be NULL; `residual_output` receives h and may be NULL, or `input` or
+ * `residual` themselves.  `output` receives bf16(y), `quantized` the MXFP8 form of that BF16 tensor
+ * (E4M3 [rows, hidden] packed, scales in native atoms, 2^0 where an atom reaches past the operand):
+ * the same bytes fuse_b200_quantize_mxfp8 makes of `output`.  One of the two at least. */
+typedef struct fuse_b200_rms_norm_params {
+  const fuse_bf16* input;
+  const fuse_bf16* residual;
+  const fuse_bf16* gamma;
+  fuse_bf16* residual_output;
+  fuse_bf16* output;
+  fuse_mxfp8_activation quantized;
+  int64_t input_stride, residual_stride, residual_output_stride, output_stride;
+  int64_t rows;
+  int32_t hidden;
+  float epsilon;
+} fuse_b200_rms_norm_params;
+FUSE_API int fuse_b200_launch_rms_norm(const fuse_b200_rms_norm_params* params, fuse_stream stream);
+
+/* Gradients of the above.  `stream_input` is h (residual_output, or input when there was no residual),
+ * `grad_stream` the gradient that reaches h past the norm (may be NULL).  grad_input receives the
+ * gradient of input and of residual alike (may be `grad_output` or `grad_stream` themselves),
+ * grad_gamma (may be NULL) the BF16 gradient of gamma, summed in FP32 in an order that only the sizes
+ * and the device fix.  `workspace` (256-byte aligned) is needed with grad_gamma. */
+typedef struct fuse_b200_rms_norm_backward_params {
+  const fuse_bf16* grad_output;
+  const fuse_bf16* stream_input;
+  const fuse_bf16* gamma;
+  const fuse_bf16* grad_stream;
+  fuse_bf16* grad_input;
+  fuse_bf16* grad_gamma;
+  int64_t grad_output_stride, stream_input_stride, grad_stream_stride, grad_input_stride;
+  int64_t rows;
+  int32_t hidden;
+  float epsilon;
+  void* workspace;
+  size_t workspace_bytes;
+} fuse_b200_rms_norm_backward_params;
+FUSE_API int fuse_b200_rms_norm_backward_workspace_size(int64_t rows, int32_t hidden, size_t* bytes);
+FUSE_API int fuse_b200_launch_rms_norm_backward(const fuse_b200_rms_norm_backward_params* params, fuse_stream stream);
+
+/* Rotary positions.  The first rotary_dim elements of every head are rotary_dim / 2 pairs: (2i, 2i + 1)
+ * when interleaved, else (i, i + rotary_dim / 2); pair i at position p is turned by p * f_i and scaled by
+ * the magnitude; the rest of the head is copied.  Frequencies (n = rotary_dim):
+ *   NONE        f_i = theta^(-2 i / n)
+ *   LINEAR      f_i / factor
+ *   NTK         theta replaced by theta * factor^(n / (n - 2))
+ *   WAVELENGTH  pairs that turn more than high_freq_factor times within original_context keep f_i, those
+ *               below low_freq_factor turns get f_i / factor, linear in the turns between
+ *   YARN        the ramp between f_i and f_i / factor is linear in i, from the pair that turns beta_fast times
+ *               within original_context to the one that turns beta_slow times; magnitude
+ *               0.1 ln(factor) + 1 unless `magnitude` says otherwise */
+enum {
+  FUSE_B200_ROTARY_NONE = 0,
+  FUSE_B200_ROTARY_LINEAR = 1,
+  FUSE_B200_ROTARY_NTK = 2,
+  FUSE_B200_ROTARY_WAVELENGTH = 3,
+  FUSE_B200_ROTARY_YARN = 4
+};
+typedef struct fuse_b200_rotary_spec {
+  double theta;
+  double factor;
+  double low_freq_factor, high_freq_factor;
+  double beta_fast, beta_slow;
+  double magnitude; /* 0: the scaling's own */
+  int64_t original_context;
+  int32_t rotary_dim; /* even, 2 .. head_dim, at most 256 */
+  int32_t scaling;
+  uint8_t interleaved;
+} fuse_b200_rotary_spec;
+/* q [rows, q_heads * head_dim], k [rows, kv_heads * head_dim]; either may be absent (NULL, no heads).
+ * Outputs may be the inputs themselves (same pointer and stride), not overlap them otherwise.  The
+ * position of row r is positions[r] (int32 or int64, position_bytes 4 or 8) or, without positions,
+ * position_start + r % seq_len.  `adjoint` turns the other way with the same magnitude: the gradient. */
+typedef struct fuse_b200_rotary_params {
+  const fuse_bf16* q;
+  const fuse_bf16* k;
+  fuse_bf16* q_output;
+  fuse_bf16* k_output;
+  int64_t q_stride, k_stride, q_output_stride, k_output_stride;
+  const void* positions;
+  int64_t position_start;
+  int64_t rows, seq_len;
+  fuse_b200_rotary_spec spec;
+  int32_t q_heads, kv_heads, head_dim;
+  int32_t position_bytes;
+  uint8_t adjoint;
+} fuse_b200_rotary_params;
+/* Host: the rotary_dim / 2 frequencies (radians per position) and the magnitude of a spec. */
+FUSE_API int fuse_b200_rotary_frequencies(const fuse_b200_rotary_spec* spec, double* frequencies, double* magnitude);
+FUSE_API int fuse_b200_launch_rotary(const fuse_b200_rotary_params* params, fuse_stream stream);
+
 /* The static tile order shared by compute and communication CTAs: linear index -> (m, n) tile
  * for a grid of m_tiles x n_tiles, swizzle in {1,2,4,8}, along_n = 0 (index runs down M inside
  * bands of `swizzle` N tiles) or 1 (transpose).  Same knobs as the reference scheduler
@@ -584,7 +684,8 @@ FUSE_API int fuse_b200_read_status(uint32_t out[16], int clear);
  * 13 mxfp8_gemm_a2a_params, 14 mxfp8_a2a_gemm_params, 15 grouped_gemm_policy,
  * 16 bf16_grouped_gemm_params, 17 mxfp8_qkv_backward_data_params, 18 mxfp8_qkv_backward_weight_params,
  * 19 mxfp8_qkv_backward_params, 20 mxfp8_oproj_backward_data_params, 21 mxfp8_oproj_backward_weight_params,
- * 22 mxfp8_oproj_backward_params.  -1 for unknown ids. */
+ * 22 mxfp8_oproj_backward_params, 23 rms_norm_params, 24 rms_norm_backward_params, 25 rotary_spec,
+ * 26 rotary_params.  -1 for unknown ids. */
 FUSE_API int fuse_b200_abi_sizeof(int record);
 /* Number of kernels this library has launched in this process (all entry points). */
 FUSE_API uint64_t fuse_b200_launch_count(void);
