@@ -308,12 +308,30 @@ class RotaryParams(C.Structure):
                 ("adjoint", C.c_uint8)]
 
 
+class AttentionParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("output", C.c_void_p), ("lse", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("output_stride", C.c_int64),
+                ("q_rows", C.c_int64), ("kv_rows", C.c_int64), ("q_starts", C.c_void_p), ("q_lengths", C.c_void_p),
+                ("kv_starts", C.c_void_p), ("kv_lengths", C.c_void_p), ("batch", C.c_int32), ("q_len", C.c_int32),
+                ("kv_len", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("window", C.c_int32), ("sinks", C.c_int32), ("causal", C.c_uint8), ("scale", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class AttentionBackwardParams(C.Structure):
+    _fields_ = [("forward", AttentionParams), ("grad_output", C.c_void_p), ("grad_q", C.c_void_p),
+                ("grad_k", C.c_void_p), ("grad_v", C.c_void_p), ("grad_output_stride", C.c_int64),
+                ("grad_q_stride", C.c_int64), ("grad_k_stride", C.c_int64), ("grad_v_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 ABI_RECORDS = {0: GemmProblem, 1: UlyssesRoute, 2: GemmA2AParams, 3: A2AGemmParams,
                4: KernelTraits, 5: Options, 17: Mxfp8QkvBackwardDataParams, 18: Mxfp8QkvBackwardWeightParams,
                19: Mxfp8QkvBackwardParams, 20: Mxfp8OprojBackwardDataParams, 21: Mxfp8OprojBackwardWeightParams,
                22: Mxfp8OprojBackwardParams, 15: GroupedGemmPolicy, 16: Bf16GroupedGemmParams, 14: Mxfp8A2AGemmParams, 12: Mxfp8Activation, 13: Mxfp8GemmA2AParams, 6: QkvBackwardDataParams, 7: QkvBackwardWeightParams,
                8: QkvBackwardParams, 9: OprojBackwardDataParams, 10: OprojBackwardWeightParams,
-               11: OprojBackwardParams, 23: RmsNormParams, 24: RmsNormBackwardParams, 25: RotarySpec, 26: RotaryParams}
+               11: OprojBackwardParams, 23: RmsNormParams, 24: RmsNormBackwardParams, 25: RotarySpec, 26: RotaryParams,
+               27: AttentionParams, 28: AttentionBackwardParams}
 
 # Every symbol include/fuse_b200.h declares: name -> (restype, argtypes).
 _P = C.c_void_p
@@ -388,6 +406,10 @@ SYMBOLS = {
     "fuse_b200_launch_rms_norm_backward": (C.c_int, [C.POINTER(RmsNormBackwardParams), _P]),
     "fuse_b200_rotary_frequencies": (C.c_int, [C.POINTER(RotarySpec), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     "fuse_b200_launch_rotary": (C.c_int, [C.POINTER(RotaryParams), _P]),
+    "fuse_b200_attention_workspace_size": (C.c_int, [C.POINTER(AttentionParams), C.POINTER(C.c_size_t)]),
+    "fuse_b200_launch_attention": (C.c_int, [C.POINTER(AttentionParams), C.POINTER(Options), _P]),
+    "fuse_b200_attention_backward_workspace_size": (C.c_int, [C.POINTER(AttentionBackwardParams), C.POINTER(C.c_size_t)]),
+    "fuse_b200_launch_attention_backward": (C.c_int, [C.POINTER(AttentionBackwardParams), C.POINTER(Options), _P]),
     "fuse_b200_generate_bf16": (C.c_int, [_P, C.c_uint64, C.c_uint64, C.c_float, C.c_int, _P]),
     "fuse_b200_tile_order_decode": (C.c_int, [C.c_int32] * 4 + [C.c_int64, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "fuse_b200_select_swizzle": (C.c_int32, [C.c_int32] * 3),

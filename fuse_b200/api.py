@@ -341,8 +341,9 @@ def launch_gemm_a2a_mxfp8_static(params: Mxfp8GemmA2AParams, stream: int = 0) ->
     return N.lib().fuse_b200_launch_gemm_a2a_mxfp8_static(C.byref(params), stream)
 
 
-# ---- block operators: residual RMS norm, rotary positions (include/fuse_b200.h) ------------------
-from ._native import RmsNormBackwardParams, RmsNormParams, RotaryParams, RotarySpec  # noqa: E402,F401
+# ---- block operators: residual RMS norm, rotary positions, attention (include/fuse_b200.h) -------
+from ._native import (AttentionBackwardParams, AttentionParams, RmsNormBackwardParams, RmsNormParams, RotaryParams,  # noqa: E402,F401
+                      RotarySpec)
 
 
 def launch_rms_norm(params: RmsNormParams, stream: int = 0) -> int:
@@ -369,3 +370,20 @@ def rotary_frequencies(spec: RotarySpec):
 
 def launch_rotary(params: RotaryParams, stream: int = 0) -> int:
     return N.lib().fuse_b200_launch_rotary(C.byref(params), stream)
+
+
+def attention_workspace_size(params: AttentionParams):
+    return _size(N.lib().fuse_b200_attention_workspace_size, params)
+
+
+def launch_attention(params: AttentionParams, stream: int = 0, options: Options | None = None) -> int:
+    """Attention with a sliding window and sinks on planar Q, K, V."""
+    return N.lib().fuse_b200_launch_attention(C.byref(params), _opt(options), stream)
+
+
+def attention_backward_workspace_size(params: AttentionBackwardParams):
+    return _size(N.lib().fuse_b200_attention_backward_workspace_size, params)
+
+
+def launch_attention_backward(params: AttentionBackwardParams, stream: int = 0, options: Options | None = None) -> int:
+    return N.lib().fuse_b200_launch_attention_backward(C.byref(params), _opt(options), stream)

@@ -286,3 +286,130 @@ def rotary_(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, hea
         raise RuntimeError("rotary_ writes its arguments and has no gradient: use rotary")
     _rotary_launch(q, k, q, k, record, head_dim, seq_len, start, positions, 0)
     return q, k
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def _attention_record(q, k, v, shape):
+    """The launch record without outputs; `shape`: the scalars every launch of this call shares."""
+    batch, q_len, kv_len, q_heads, kv_heads, head_dim, causal, window, sinks, scale, q_starts, q_lengths, kv_starts, kv_lengths = shape
+    p = N.AttentionParams()
+    p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    p.q_stride, p.k_stride, p.v_stride = _stride(q), _stride(k), _stride(v)
+    p.q_rows, p.kv_rows = q.shape[0], k.shape[0]
+    if q_starts is not None:
+        p.q_starts = q_starts.data_ptr()
+    if q_lengths is not None:
+        p.q_lengths = q_lengths.data_ptr()
+    if kv_starts is not None:
+        p.kv_starts = kv_starts.data_ptr()
+    if kv_lengths is not None:
+        p.kv_lengths = kv_lengths.data_ptr()
+    p.batch, p.q_len, p.kv_len = batch, q_len, kv_len
+    p.q_heads, p.kv_heads, p.head_dim = q_heads, kv_heads, head_dim
+    p.causal, p.window, p.sinks, p.scale = causal, window, sinks, scale
+    return p
+
+
+def _partial(q, k, shape) -> bool:
+    """Whether some rows may belong to no sequence."""
+    return any(t is not None for t in shape[10:]) or shape[0] * shape[1] != q.shape[0] or shape[0] * shape[2] != k.shape[0]
+
+
+def _attention_forward(q, k, v, shape, out, want_lse):
+    ragged = _partial(q, k, shape)
+    if out is None:  # rows of no sequence are zeros here; the operator leaves them as they are
+        out = (torch.zeros if ragged else torch.empty)(q.shape, dtype=BF16, device=q.device)
+    p = _attention_record(q, k, v, shape)
+    p.output, p.output_stride = out.data_ptr(), _stride(out)
+    lse = None
+    if want_lse:
+        lse = torch.full((shape[3], q.shape[0]), -torch.inf, dtype=torch.float32, device=q.device) if ragged else \
+            torch.empty((shape[3], q.shape[0]), dtype=torch.float32, device=q.device)
+        p.lse = lse.data_ptr()
+    with _On(q) as stream:
+        size = C.c_size_t()
+        _check(N.lib().fuse_b200_attention_workspace_size(C.byref(p), C.byref(size)), "attention_workspace_size")
+        if size.value:
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device)
+            p.workspace, p.workspace_bytes = workspace.data_ptr(), size.value
+        _check(N.lib().fuse_b200_launch_attention(C.byref(p), None, stream), "launch_attention")
+    return out, lse
+
+
+def _attention_backward(do, q, k, v, out, lse, shape):
+    make = torch.zeros if _partial(q, k, shape) or not q.shape[0] else torch.empty
+    dq, dk, dv = (make(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
+    if not q.shape[0]:
+        return dq, dk, dv
+    do = _grad(do)
+    p = N.AttentionBackwardParams()
+    p.forward = _attention_record(q, k, v, shape)
+    p.forward.output, p.forward.output_stride, p.forward.lse = out.data_ptr(), _stride(out), lse.data_ptr()
+    p.grad_output, p.grad_output_stride = do.data_ptr(), _stride(do)
+    p.grad_q, p.grad_k, p.grad_v = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    p.grad_q_stride = p.grad_k_stride = p.grad_v_stride = -1
+    with _On(q) as stream:
+        size = C.c_size_t()
+        _check(N.lib().fuse_b200_attention_backward_workspace_size(C.byref(p), C.byref(size)),
+               "attention_backward_workspace_size")
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = workspace.data_ptr(), size.value
+        _check(N.lib().fuse_b200_launch_attention_backward(C.byref(p), None, stream), "launch_attention_backward")
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, shape):
+        out, lse = _attention_forward(q, k, v, shape, None, True)
+        ctx.save_for_backward(q, k, v, out, lse, *shape[10:])
+        ctx.shape = shape[:10]
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, _lse):
+        q, k, v, out, lse, *rows = ctx.saved_tensors
+        dq, dk, dv = _attention_backward(do, q, k, v, out, lse, (*ctx.shape, *rows))
+        return dq, dk, dv, None
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: int, batch: int = 1, causal: bool = True,
+              window: int = 0, sinks: int = 0, scale: float | None = None, q_len: int | None = None,
+              kv_len: int | None = None, q_starts: torch.Tensor | None = None, q_lengths: torch.Tensor | None = None,
+              kv_starts: torch.Tensor | None = None, kv_lengths: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, return_lse: bool = False):
+    """softmax(scale q k^T) v per head: q [rows, q_heads * head_dim], k and v [kv_rows, kv_heads * head_dim] -> like q.
+
+    The rows are `batch` sequences of q_len queries and kv_len keys (default: all rows, evenly), one behind the other.
+    Shorter ones have their lengths in q_lengths / kv_lengths, others their first rows in q_starts / kv_starts
+    (int32 [batch] on the device; q_len and kv_len are then the longest).  Queries are the last q_length
+    positions of their sequence.  With `causal`, `window` limits a query to the last `window` keys up to its own and the
+    first `sinks` of the sequence.  Rows of no sequence are zeros in the result (with `out`: as they were).
+    `out`: a tensor to write to, such as UlyssesProjections.attention_buffer() -- without gradients only, since a
+    later call would overwrite what the backward needs.  `return_lse`: also FP32 [q_heads, rows], no gradient."""
+    _rows(q, "q")
+    _rows(k, "k", device=q.device)
+    _rows(v, "v", k.shape[1], k.shape[0], q.device)
+    if head_dim <= 0 or q.shape[1] % head_dim or k.shape[1] % head_dim or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"heads of {head_dim}: rows of {q.shape[1]} (q) and {k.shape[1]} (k, v) elements are not whole groups")
+    if batch <= 0 or (q_len is None and q.shape[0] % batch) or (kv_len is None and k.shape[0] % batch):
+        raise ValueError(f"{q.shape[0]} queries and {k.shape[0]} keys are not {batch} sequences")
+    for t, name in ((q_starts, "q_starts"), (q_lengths, "q_lengths"), (kv_starts, "kv_starts"), (kv_lengths, "kv_lengths")):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous() or t.device != q.device):
+            raise ValueError(f"{name}: expected contiguous int32 ({batch},) on {q.device}")
+    if window < 0 or sinks < 0 or (window and not causal):
+        raise ValueError("window and sinks are not negative, and a window goes with causal attention")
+    shape = (batch, q.shape[0] // batch if q_len is None else q_len, k.shape[0] // batch if kv_len is None else kv_len,
+             q.shape[1] // head_dim, k.shape[1] // head_dim, head_dim, 1 if causal else 0, window, sinks,
+             head_dim ** -0.5 if scale is None else scale, q_starts, q_lengths, kv_starts, kv_lengths)
+    if out is not None:
+        _rows(out, "out", q.shape[1], q.shape[0], q.device)
+    if _wants_grad(q, k, v):
+        if out is not None:
+            raise RuntimeError("out= would be overwritten before the backward has read it: leave it out, or use torch.no_grad()")
+        out, lse = _Attention.apply(q, k, v, shape)
+    else:
+        out, lse = _attention_forward(q, k, v, shape, out, return_lse)
+    return (out, lse) if return_lse else out

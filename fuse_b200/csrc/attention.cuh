@@ -1,0 +1,515 @@
+// Attention with a sliding window and visible first tokens (sinks), forward: one CTA works on two 128-row
+// tiles of queries against the keys they can see.
+//
+//   S = scale Q K^T over the visible keys, m = max S, P = exp(S - m), l = sum P, O = P V / l, lse = m + log l
+//
+// Query i of a sequence is at position p = i + kv_length - q_length and sees keys j <= p with p - j < window
+// or j < sinks.  Key tiles that no row of the pair of tiles sees are not visited: the sinks' tiles come first,
+// then the window's.
+//
+// A tile's 128 rows are `pack` query heads that share a KV head times 128 / pack tokens (heads fastest):
+// the tensor map's box brings them in that order.  A group of heads then reads each key tile once, and a few
+// new tokens of many heads still fill rows.
+//
+// Roles (12 warps): warp 0 loads (TMA: both Q tiles, then K and V tiles through two rings), warp 1 issues the
+// UMMAs, warp 2 allocates TMEM, warps 4-7 and 8-11 are one softmax group per tile, one thread per row.
+// TMEM (512 columns): S of either tile (128 FP32 columns each; P overwrites the first 64 of its own S as
+// packed BF16 and is the A operand of P V straight from there) and O of either tile.
+//
+// The UMMA order is P V of tile 0, S of tile 0 for the next keys, then the same for tile 1: while one tile's
+// softmax runs, the tensor cores work for the other.  The UMMAs of a CTA execute in issue order, so S may
+// overwrite the P that the UMMA before it reads, and "S of the next keys is complete" implies "O holds all
+// keys before", which is what a softmax group needs to rescale O in place.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then
+// stay below 2^8 in BF16 and the sums below 2^8 kv_len in FP32; the result is divided by the same sum, so
+// this changes no value beyond rounding).  S, the statistics and O are FP32; P is rounded to BF16 for the
+// second product and summed before that rounding.
+#pragma once
+
+#include "host.cuh"
+#include "sync.cuh"
+
+namespace fuse_b200 {
+namespace attn {
+
+constexpr int kTile = 128;  // rows of a query tile, keys of a key tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Args {
+  WaitContext wait;
+  const int32_t *q_starts, *q_lengths, *kv_starts, *kv_lengths;
+  int64_t q_rows, kv_rows;  // extents of the tensors
+  int32_t batch, q_len, kv_len, q_heads, kv_heads;
+  int32_t pack;        // query heads in a tile: a power of two that divides the group
+  int32_t pack_shift;
+  int32_t causal, window, sinks;
+  float scale, scale_log2;
+  uint16_t* out;
+  int64_t out_stride;
+  float* lse;  // [q_heads][q_rows] or nullptr
+  // split over keys: partial results per (split, batch, token, head), joined by a second kernel
+  int32_t splits;
+  float *partial, *partial_lse;
+};
+
+struct Sequence {
+  int32_t q0, k0;  // first rows
+  int32_t ql, kl;  // lengths
+  int32_t off;     // position of query 0
+};
+
+// Lengths and starts come from device memory: whatever they hold, no row outside the tensors is touched.
+__device__ __forceinline__ void clamp_rows(int64_t start, int32_t length, int32_t most, int64_t rows, int32_t* first,
+                                           int32_t* count) {
+  int64_t n = length < most ? length : most;
+  if (start < 0 || start > rows) n = start = 0;
+  if (n > rows - start) n = rows - start;
+  *first = int32_t(start);
+  *count = n < 0 ? 0 : int32_t(n);
+}
+__device__ __forceinline__ Sequence sequence(const Args& a, int32_t b) {
+  Sequence s;
+  clamp_rows(a.q_starts ? a.q_starts[b] : int64_t(b) * a.q_len, a.q_lengths ? a.q_lengths[b] : a.q_len, a.q_len, a.q_rows,
+             &s.q0, &s.ql);
+  clamp_rows(a.kv_starts ? a.kv_starts[b] : int64_t(b) * a.kv_len, a.kv_lengths ? a.kv_lengths[b] : a.kv_len, a.kv_len,
+             a.kv_rows, &s.k0, &s.kl);
+  s.off = s.kl - s.ql;
+  return s;
+}
+
+// What the tokens [first, last) of a sequence see: keys [lo, end) and [0, sinks).
+struct KeyRange {
+  int32_t lo, end, sinks;
+  __device__ __forceinline__ KeyRange(const Args& a, const Sequence& s, int32_t first, int32_t last) {
+    lo = 0;
+    end = s.kl;
+    if (a.causal) {
+      if (last + s.off < end) end = last + s.off;
+      if (a.window > 0 && first + s.off - a.window + 1 > 0) lo = first + s.off - a.window + 1;
+    }
+    if (first >= last || end < 0) end = 0;
+    sinks = a.window > 0 && a.sinks > 0 ? (a.sinks < end ? a.sinks : end) : 0;
+  }
+  __device__ __forceinline__ bool sees(int32_t tile) const {
+    return tile * kTile < end && ((tile + 1) * kTile > lo || tile * kTile < sinks);
+  }
+};
+// Tiles of a range in the order they are visited.
+struct TileList {
+  int32_t sink_tiles, first, count;
+  __device__ __forceinline__ explicit TileList(const KeyRange& r) {
+    first = r.lo / kTile;
+    sink_tiles = (r.sinks + kTile - 1) / kTile;
+    if (sink_tiles > first) sink_tiles = first;
+    count = r.end > 0 ? sink_tiles + (r.end + kTile - 1) / kTile - first : 0;
+  }
+  __device__ __forceinline__ int32_t tile(int32_t i) const { return i < sink_tiles ? i : first + i - sink_tiles; }
+};
+// Whether some row among tokens [first, last) does not see all of a key tile.
+__device__ __forceinline__ bool needs_mask(const Args& a, const Sequence& s, int32_t first, int32_t last, int32_t tile) {
+  const int32_t k0 = tile * kTile;
+  if (k0 + kTile > s.kl) return true;
+  if (!a.causal) return false;
+  if (k0 + kTile - 1 > first + s.off) return true;
+  return a.window > 0 && k0 < last - 1 + s.off - a.window + 1 && k0 + kTile > a.sinks;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitContext& w, uint32_t site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, site));
+}
+
+// A [128 x kDim] BF16 tile in shared memory: kDim / 64 blocks of 128 rows x 128 bytes, 128-byte swizzle.
+template <int kDim>
+struct TileShape {
+  static constexpr uint32_t kBlockBytes = kTile * 128;
+  static constexpr uint32_t kBlocks = kDim / 64;
+  static constexpr uint32_t kBytes = kBlocks * kBlockBytes;
+};
+template <int kDim>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t head, int32_t row) {
+#pragma unroll
+  for (uint32_t b = 0; b < TileShape<kDim>::kBlocks; ++b)
+    ptx::tma_load_3d(dst + b * TileShape<kDim>::kBlockBytes, map, bar, int32_t(b * 64), head, row);
+}
+// Rows [valid, 128) of a tile become zeros (a row is 128 bytes in every block, whatever the swizzle): what lies
+// behind a sequence's end may be anything, and 0 times that need not be 0.  One row per thread.
+template <int kDim>
+__device__ __forceinline__ void zero_rows(uint32_t tile, int32_t row, int32_t valid) {
+  if (row >= valid) {
+#pragma unroll
+    for (uint32_t b = 0; b < TileShape<kDim>::kBlocks; ++b)
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)
+        ptx::st_shared_v4(tile + b * TileShape<kDim>::kBlockBytes + uint32_t(row) * 128u + i * 16u, make_uint4(0u, 0u, 0u, 0u));
+  }
+  ptx::fence_proxy_async_shared();
+}
+
+// D[128 x 128] = A B^T over kDim: both operands K-major tiles (rows of A, rows of B).
+template <int kDim>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile) {
+  constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kTile, 0, 0);
+#pragma unroll
+  for (uint32_t k = 0; k < kDim / 16; ++k) {
+    const uint32_t at = (k / 4) * TileShape<kDim>::kBlockBytes + (k % 4) * 32;
+    ptx::umma_f16(d, ptx::smem_desc_k_sw128(a_tile + at), ptx::smem_desc_k_sw128(b_tile + at), kIdesc, k != 0 ? 1u : 0u);
+  }
+}
+// D[128 x kDim] (+)= A[128 x 128] B: A in TMEM (K values 16 k .. 16 k + 15 at column a_column(k)), B a tile whose rows
+// are the K axis.
+template <int kDim, class Column>
+__device__ __forceinline__ void mma_weights(uint32_t d, Column a_column, uint32_t b_tile, bool accumulate) {
+  constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kDim, 0, 1);
+#pragma unroll
+  for (uint32_t k = 0; k < kTile / 16; ++k)
+    ptx::umma_f16_a_tmem(d, a_column(k), ptx::smem_desc_mn_sw128(b_tile + k * 2048u, TileShape<kDim>::kBlockBytes), kIdesc,
+                         accumulate || k != 0 ? 1u : 0u);
+}
+
+template <int kDim>
+struct ForwardLayout {
+  static constexpr int kStages = kDim == 128 ? 2 : 4;  // of either ring
+  static constexpr uint32_t kTileBytes = TileShape<kDim>::kBytes;
+  static constexpr uint32_t kK = 2 * kTileBytes;
+  static constexpr uint32_t kV = kK + kStages * kTileBytes;
+  static constexpr uint32_t kBarriers = kV + kStages * kTileBytes;
+  // q_full[2], s_full[2], p_ready[2], o_full, drain, then k_full, k_empty, v_full, v_empty [kStages]
+  static constexpr uint32_t kNumBarriers = 8 + 4 * kStages;
+  static constexpr uint32_t kSlot = kBarriers + kNumBarriers * 8;
+  static constexpr uint32_t kDynamicBytes = kSlot + 16 + 1024;
+  static_assert(kDynamicBytes <= 227 * 1024, "shared memory budget");
+  static_assert(kDynamicBytes > 114 * 1024, "must force one CTA per SM (all of TMEM is allocated)");
+};
+constexpr int kForwardThreads = 384;
+
+template <int kDim>
+__global__ void __launch_bounds__(kForwardThreads, 1)
+attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
+  using Layout = ForwardLayout<kDim>;
+  constexpr int kStages = Layout::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // block -> (tokens, head pack, batch, split); the last tokens, which see the most keys, come first
+  const int32_t tile_tokens = kTile >> a.pack_shift, packs = a.q_heads >> a.pack_shift;
+  int32_t at = int32_t(blockIdx.x);
+  const int32_t split = at % a.splits;
+  at /= a.splits;
+  const int32_t pack = at % packs;
+  at /= packs;
+  const int32_t b = at % a.batch;
+  const int32_t token_blocks = (a.q_len + 2 * tile_tokens - 1) / (2 * tile_tokens);
+  const int32_t t0 = (token_blocks - 1 - at / a.batch) * 2 * tile_tokens;
+  const Sequence seq = sequence(a, b);
+  if (t0 >= seq.ql) return;  // (the whole block, before anything is set up)
+  const int32_t head0 = pack << a.pack_shift, kv_head = head0 / (a.q_heads / a.kv_heads);
+  const int32_t first[2] = {t0, t0 + tile_tokens};
+  const int32_t last[2] = {min(t0 + tile_tokens, seq.ql), min(t0 + 2 * tile_tokens, seq.ql)};
+  const KeyRange range(a, seq, t0, last[1]);
+  const KeyRange own[2] = {KeyRange(a, seq, first[0], last[0]), KeyRange(a, seq, first[1], last[1])};
+  const TileList tiles(range);
+  const int32_t per_split = (tiles.count + a.splits - 1) / a.splits;
+  const int32_t it0 = min(split * per_split, tiles.count), it1 = min(it0 + per_split, tiles.count);
+
+  const uint32_t bars = base + Layout::kBarriers;
+  auto q_full = [&](int t) { return bars + 8u * t; };
+  auto s_full = [&](int t) { return bars + 8u * (2 + t); };
+  auto p_ready = [&](int t) { return bars + 8u * (4 + t); };
+  const uint32_t o_full = bars + 8u * 6, drain = bars + 8u * 7;
+  auto k_full = [&](int s) { return bars + 8u * (8 + s); };
+  auto k_empty = [&](int s) { return bars + 8u * (8 + kStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (8 + 2 * kStages + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (8 + 3 * kStages + s); };
+  auto k_tile = [&](int s) { return base + Layout::kK + s * Layout::kTileBytes; };
+  auto v_tile = [&](int s) { return base + Layout::kV + s * Layout::kTileBytes; };
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&map_q);
+    ptx::prefetch_tensormap(&map_k);
+    ptx::prefetch_tensormap(&map_v);
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(q_full(t), 1);
+      ptx::mbar_init(s_full(t), 1);
+      ptx::mbar_init(p_ready(t), 4);  // one arrival per warp of the softmax group
+    }
+    ptx::mbar_init(o_full, 1);
+    ptx::mbar_init(drain, 1);
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(k_full(s), 1);
+      ptx::mbar_init(k_empty(s), 1);
+      ptx::mbar_init(v_full(s), 1);
+      ptx::mbar_init(v_empty(s), 1);
+    }
+    ptx::fence_mbar_init();
+  }
+  if (warp == 2) {
+    ptx::tmem_alloc(base + Layout::kSlot, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (base - raw) + Layout::kSlot);
+  auto s_tmem = [&](int t) { return tmem + uint32_t(t) * 128u; };
+  auto o_tmem = [&](int t) { return tmem + 256u + uint32_t(t) * 128u; };
+
+  bool unwound = false;
+  if (warp == 0) {
+    if (lane == 0 && it0 < it1) {
+      bool ok = true;
+      auto load_q = [&](int t) {
+        if (first[t] >= last[t]) return;
+        ptx::mbar_expect_tx(q_full(t), Layout::kTileBytes);
+        load_tile<kDim>(base + t * Layout::kTileBytes, &map_q, q_full(t), head0, seq.q0 + first[t]);
+      };
+      load_q(0);
+      for (int32_t it = it0; ok && it < it1; ++it) {
+        const int s = (it - it0) % kStages;
+        const uint32_t phase = ((it - it0) / kStages) & 1;
+        const int32_t row = seq.k0 + tiles.tile(it) * kTile;
+        if (!(ok = mbar_wait(k_empty(s), phase ^ 1u, a.wait, kSiteSmemEmpty))) break;
+        ptx::mbar_expect_tx(k_full(s), Layout::kTileBytes);
+        load_tile<kDim>(k_tile(s), &map_k, k_full(s), kv_head, row);
+        if (it == it0) load_q(1);
+        if (!(ok = mbar_wait(v_empty(s), phase ^ 1u, a.wait, kSiteSmemEmpty))) break;
+        ptx::mbar_expect_tx(v_full(s), Layout::kTileBytes);
+        load_tile<kDim>(v_tile(s), &map_v, v_full(s), kv_head, row);
+      }
+      unwound = !ok;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && it0 < it1) {
+      bool ok = true, started[2] = {false, false};
+      uint32_t p_phase[2] = {0, 0};
+      auto scores = [&](int t, int32_t it) {  // S of tile t; K of `it` has arrived
+        if (!started[t] && !(ok = mbar_wait(q_full(t), 0, a.wait, kSiteSmemFull))) return;
+        mma_rows<kDim>(s_tmem(t), base + t * Layout::kTileBytes, k_tile((it - it0) % kStages));
+        ptx::umma_commit(s_full(t));
+        started[t] = true;
+      };
+      bool has_o[2] = {false, false};
+      for (int32_t it = it0 - 1; ok && it < it1; ++it) {
+        const bool now = it >= it0, next = it + 1 < it1;
+        const int s = (it - it0) % kStages;
+        const int32_t tile = now ? tiles.tile(it) : 0, next_tile = next ? tiles.tile(it + 1) : 0;
+        bool have_v = false, have_k = false;
+        for (int t = 0; ok && t < 2; ++t) {
+          if (now && own[t].sees(tile)) {
+            if (!(ok = mbar_wait(p_ready(t), p_phase[t], a.wait, kSiteTmemEmpty))) break;
+            p_phase[t] ^= 1u;
+            if (!have_v && !(ok = mbar_wait(v_full(s), ((it - it0) / kStages) & 1, a.wait, kSiteSmemFull))) break;
+            have_v = true;
+            ptx::tc_fence_after();
+            mma_weights<kDim>(o_tmem(t), [&](uint32_t k) { return s_tmem(t) + k * 8u; }, v_tile(s), has_o[t]);
+            has_o[t] = true;
+          }
+          if (next && own[t].sees(next_tile)) {
+            if (!have_k && !(ok = mbar_wait(k_full((it + 1 - it0) % kStages), ((it + 1 - it0) / kStages) & 1, a.wait, kSiteSmemFull)))
+              break;
+            have_k = true;
+            scores(t, it + 1);
+          }
+        }
+        if (!ok) break;
+        if (now) ptx::umma_commit(v_empty(s));
+        if (next) ptx::umma_commit(k_empty((it + 1 - it0) % kStages));
+      }
+      if (ok) {
+        ptx::umma_commit(o_full);
+      } else {
+        ptx::umma_commit(drain);  // UMMAs already issued retire before TMEM is released
+        mbar_wait(drain, 0u, a.wait, kSiteDrain, false);
+      }
+      unwound = !ok;
+    }
+  } else if (warp >= 4) {
+    const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_at = s_tmem(t) + lanes, o_at = o_tmem(t) + lanes;
+    const int32_t token = first[t] + (row >> a.pack_shift), head = head0 + (row & (a.pack - 1));
+    const int32_t pos = token + seq.off;
+    const int32_t hi = a.causal ? min(pos, seq.kl - 1) : seq.kl - 1;
+    const int32_t lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
+    const int32_t sinks = a.window > 0 ? a.sinks : 0;
+    const bool live = first[t] < last[t];
+    float m = -INFINITY, l = 0.0f;  // m: the reference of the exponent, in units of the scaled score's log2
+    bool ok = true, begun = false;
+    uint32_t phase = 0;
+    for (int32_t it = it0; ok && it < it1; ++it) {
+      const int32_t tile = tiles.tile(it);
+      if (!own[t].sees(tile)) continue;
+      if (!(ok = warp_wait(s_full(t), phase, a.wait, kSiteTmemFull))) break;
+      ptx::tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(s_at + i * 32, s[i]);
+      ptx::tmem_wait_ld();
+      if (needs_mask(a, seq, first[t], last[t], tile)) {
+        const int32_t k0 = tile * kTile, h = hi - k0, w = lo - k0, n = sinks - k0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int32_t key = i * 32 + c;
+            if (!(key <= h && (key >= w || key < n))) s[i][c] = 0xff800000u;
+          }
+      }
+      float top[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        top[i] = as_float(s[i][0]);
+#pragma unroll
+        for (int c = 1; c < 32; ++c) top[i] = fmaxf(top[i], as_float(s[i][c]));
+      }
+      const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+      if (__any_sync(0xffffffffu, largest > m + 8.0f)) {
+        const float to = fmaxf(m, largest);
+        const float factor = m == -INFINITY ? 0.0f : exp2_approx(m - to);
+        l *= factor;
+        m = to;
+        if (begun) {
+          // O of the keys before is complete: S of this tile was issued behind it
+#pragma unroll
+          for (int c = 0; c < kDim; c += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(o_at + c, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(as_float(o[i]) * factor);
+            ptx::tmem_st_32x32b_x32(o_at + c, o);
+          }
+        }
+      }
+      phase ^= 1u;
+      begun = true;
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t p[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float x = exp2_approx(fmaf(as_float(s[i][2 * c]), a.scale_log2, -ref));
+          const float y = exp2_approx(fmaf(as_float(s[i][2 * c + 1]), a.scale_log2, -ref));
+          sum[i] += x + y;
+          p[c] = pack_bf16(x, y);
+        }
+        ptx::tmem_st_32x32b_x16(s_at + i * 16, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (tile * kTile + kTile > seq.kl) {  // values behind the last key (the same for the whole group)
+        const int s_v = (it - it0) % kStages;
+        if (!(ok = warp_wait(v_full(s_v), ((it - it0) / kStages) & 1, a.wait, kSiteSmemFull))) break;
+        zero_rows<kDim>(v_tile(s_v), row, seq.kl - tile * kTile);
+      }
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(p_ready(t));
+    }
+    if (ok && live) {
+      const bool any = it0 < it1;
+      if (any) ok = warp_wait(o_full, 0, a.wait, kSiteTmemFull);
+      ptx::tc_fence_after();
+      const bool mine = token < last[t];
+      const bool seen = any && l != 0.0f;  // else a row with no visible key (of this split): zeros, -inf
+      const float inverse = 1.0f / l;
+      const float lse = seen ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      const int64_t out_row = int64_t(seq.q0) + token;
+      if (ok) {
+        const int64_t cell = ((int64_t(split) * a.batch + b) * a.q_len + token) * a.q_heads + head;
+        if (mine) {
+          if (a.splits > 1) a.partial_lse[cell] = lse;
+          else if (a.lse != nullptr) a.lse[int64_t(head) * a.q_rows + out_row] = lse;
+        }
+#pragma unroll
+        for (int c = 0; c < kDim; c += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32b_x32(o_at + c, o);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = seen ? __float_as_uint(as_float(o[i]) * inverse) : 0u;
+          if (!mine) continue;
+          if (a.splits > 1) {
+            uint4* to = reinterpret_cast<uint4*>(a.partial + cell * kDim + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+            uint4* to = reinterpret_cast<uint4*>(a.out + out_row * a.out_stride + int64_t(head) * kDim + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              to[i] = make_uint4(pack_bf16(as_float(o[8 * i]), as_float(o[8 * i + 1])),
+                                 pack_bf16(as_float(o[8 * i + 2]), as_float(o[8 * i + 3])),
+                                 pack_bf16(as_float(o[8 * i + 4]), as_float(o[8 * i + 5])),
+                                 pack_bf16(as_float(o[8 * i + 6]), as_float(o[8 * i + 7])));
+          }
+        }
+      }
+    }
+    unwound = !ok;
+  }
+  if (unwound) {  // a wait gave up: loads in flight get their time to land before shared memory goes away
+    const uint64_t start = ptx::globaltimer();
+    while (ptx::globaltimer() - start < 200000ull) __nanosleep(1000);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the splits: one warp per (token, head).
+//   m = max lse_s, w_s = exp(lse_s - m), O = sum w_s O_s / sum w_s, lse = m + log sum w_s
+template <int kDim>
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ Args a) {
+  constexpr int kEach = kDim / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t cells = int64_t(a.batch) * a.q_len * a.q_heads;
+  const int64_t cell = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (cell >= cells) return;
+  const int32_t head = int32_t(cell % a.q_heads), token = int32_t(cell / a.q_heads % a.q_len);
+  const Sequence seq = sequence(a, int32_t(cell / a.q_heads / a.q_len));
+  if (token >= seq.ql) return;
+  float m = -INFINITY;
+  for (int32_t s = lane; s < a.splits; s += 32) m = fmaxf(m, a.partial_lse[s * cells + cell]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float sum = 0.0f, acc[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) acc[i] = 0.0f;
+  const float ref = m == -INFINITY ? 0.0f : m;
+  for (int32_t s = 0; s < a.splits; ++s) {
+    const float w = exp2_approx((a.partial_lse[s * cells + cell] - ref) * kLog2e);
+    if (w == 0.0f) continue;  // (the same for the whole warp)
+    sum += w;
+    const float* from = a.partial + (s * cells + cell) * kDim + lane * kEach;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) acc[i] = fmaf(w, from[i], acc[i]);
+  }
+  const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+  const int64_t row = int64_t(seq.q0) + token;
+  uint16_t* to = a.out + row * a.out_stride + int64_t(head) * kDim + lane * kEach;
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack_bf16(acc[i] * inverse, acc[i + 1] * inverse);
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[int64_t(head) * a.q_rows + row] = sum != 0.0f ? m + logf(sum) : -INFINITY;
+}
+
+}  // namespace attn
+}  // namespace fuse_b200

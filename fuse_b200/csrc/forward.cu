@@ -442,6 +442,8 @@ int fuse_b200_abi_sizeof(int record) {
     case 24: return int(sizeof(fuse_b200_rms_norm_backward_params));
     case 25: return int(sizeof(fuse_b200_rotary_spec));
     case 26: return int(sizeof(fuse_b200_rotary_params));
+    case 27: return int(sizeof(fuse_b200_attention_params));
+    case 28: return int(sizeof(fuse_b200_attention_backward_params));
     default: return -1;
   }
 }

@@ -111,6 +111,24 @@ cudaError_t encode_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMap
   return result == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t encode_tensor_map_heads(CUtensorMap* map, const void* base, uint64_t rows, uint64_t heads, uint64_t width,
+                                    uint64_t row_pitch_bytes, uint32_t box_rows, uint32_t box_heads) {
+  EncodeTiled encode = encode_entry();
+  if (encode == nullptr) return cudaErrorNotSupported;
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0 || row_pitch_bytes % 16 != 0 || (width * 2) % 16 != 0 ||
+      box_rows > 256 || box_heads > 256)
+    return cudaErrorInvalidValue;
+  const cuuint64_t dims[3] = {width, heads, rows};
+  const cuuint64_t strides[2] = {width * 2, row_pitch_bytes};
+  const cuuint32_t box[3] = {64, box_heads, box_rows};
+  const cuuint32_t element_strides[3] = {1, 1, 1};
+  const CUresult result =
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, element_strides,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return result == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 }  // namespace host
 }  // namespace fuse_b200
 

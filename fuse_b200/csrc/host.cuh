@@ -36,6 +36,11 @@ cudaError_t encode_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMap
                                  uint64_t row_pitch_bytes, uint32_t box_rows, uint32_t box_cols,
                                  CUtensorMapSwizzle swizzle);
 
+// 3-D BF16 tensor [rows, heads, width] (width contiguous), boxed [box_rows, box_heads, 64] with 128-byte
+// swizzle: what a box covers arrives as box_rows * box_heads rows of 128 bytes, heads fastest.
+cudaError_t encode_tensor_map_heads(CUtensorMap* map, const void* base, uint64_t rows, uint64_t heads, uint64_t width,
+                                    uint64_t row_pitch_bytes, uint32_t box_rows, uint32_t box_heads);
+
 inline WaitContext make_wait(const DeviceInfo& info, uint32_t epoch, uint64_t budget_ns) {
   WaitContext w;
   w.status = info.status;

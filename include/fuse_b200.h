@@ -650,6 +650,61 @@ typedef struct fuse_b200_rotary_params {
 FUSE_API int fuse_b200_rotary_frequencies(const fuse_b200_rotary_spec* spec, double* frequencies, double* magnitude);
 FUSE_API int fuse_b200_launch_rotary(const fuse_b200_rotary_params* params, fuse_stream stream);
 
+/* Attention of q_len queries per sequence over kv_len keys, between the two all-to-alls: q
+ * [q_rows, q_heads * head_dim], k and v [kv_rows, kv_heads * head_dim], output like q -- the [rows, heads * d]
+ * tensor the output projection reads.  head_dim 64 or 128; q_heads a multiple of kv_heads (query head h reads
+ * KV head h / (q_heads / kv_heads)).  Strides multiples of 8, pointers 16-byte aligned.
+ *
+ * Sequence b has q_lengths[b] <= q_len queries from row q_starts[b] on and kv_lengths[b] <= kv_len keys from row
+ * kv_starts[b] on (device int32; NULL: q_len rows from b * q_len, kv_len rows from b * kv_len).  Its query i is
+ * at position p = i + kv_length - q_length; with `causal` it sees keys j <= p, and of them, when window > 0, those
+ * with p - j < window or j < sinks.  A query that sees no key gets zeros and lse -inf.  Rows of no sequence are
+ * neither read into a result nor written; what lies behind a sequence's last row does not matter, but a NaN or
+ * infinity in a key or value of the sequence itself may reach queries that do not see it.
+ *
+ * `lse` (may be NULL): FP32 [q_heads][q_rows], log of the sum of exp(scale q k) -- what the backward needs.
+ * `workspace` (256-byte aligned, fuse_b200_attention_workspace_size; may be 0 bytes) holds partial results when
+ * the keys are split because the queries alone would leave SMs idle; two launches that may run at the same
+ * time need two. */
+typedef struct fuse_b200_attention_params {
+  const fuse_bf16* q;
+  const fuse_bf16* k;
+  const fuse_bf16* v;
+  fuse_bf16* output;
+  float* lse;
+  int64_t q_stride, k_stride, v_stride, output_stride;
+  int64_t q_rows, kv_rows;
+  const int32_t *q_starts, *q_lengths, *kv_starts, *kv_lengths;
+  int32_t batch, q_len, kv_len;
+  int32_t q_heads, kv_heads, head_dim;
+  int32_t window, sinks; /* 0: no window */
+  uint8_t causal;
+  float scale; /* > 0 */
+  void* workspace;
+  size_t workspace_bytes;
+} fuse_b200_attention_params;
+FUSE_API int fuse_b200_attention_workspace_size(const fuse_b200_attention_params* params, size_t* bytes);
+FUSE_API int fuse_b200_launch_attention(const fuse_b200_attention_params* params, const fuse_b200_options* options,
+                                        fuse_stream stream);
+
+/* Gradients of the above.  `forward`: the forward's record, with its output and lse as inputs (its workspace is not
+ * used).  grad_q like q, grad_k and grad_v like k: rows of the sequences are written, others left as they
+ * were; none of them may overlap an input.  No atomics: the same inputs give the same bits.
+ * workspace: 256-byte aligned, fuse_b200_attention_backward_workspace_size bytes. */
+typedef struct fuse_b200_attention_backward_params {
+  fuse_b200_attention_params forward;
+  const fuse_bf16* grad_output;
+  fuse_bf16* grad_q;
+  fuse_bf16* grad_k;
+  fuse_bf16* grad_v;
+  int64_t grad_output_stride, grad_q_stride, grad_k_stride, grad_v_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} fuse_b200_attention_backward_params;
+FUSE_API int fuse_b200_attention_backward_workspace_size(const fuse_b200_attention_backward_params* params, size_t* bytes);
+FUSE_API int fuse_b200_launch_attention_backward(const fuse_b200_attention_backward_params* params,
+                                                 const fuse_b200_options* options, fuse_stream stream);
+
 /* The static tile order shared by compute and communication CTAs: linear index -> (m, n) tile
  * for a grid of m_tiles x n_tiles, swizzle in {1,2,4,8}, along_n = 0 (index runs down M inside
  * bands of `swizzle` N tiles) or 1 (transpose).  Same knobs as the reference scheduler
@@ -685,7 +740,8 @@ FUSE_API int fuse_b200_read_status(uint32_t out[16], int clear);
  * 16 bf16_grouped_gemm_params, 17 mxfp8_qkv_backward_data_params, 18 mxfp8_qkv_backward_weight_params,
  * 19 mxfp8_qkv_backward_params, 20 mxfp8_oproj_backward_data_params, 21 mxfp8_oproj_backward_weight_params,
  * 22 mxfp8_oproj_backward_params, 23 rms_norm_params, 24 rms_norm_backward_params, 25 rotary_spec,
- * 26 rotary_params.  -1 for unknown ids. */
+ * 26 rotary_params, 27 attention_params, 28 attention_backward_params.
+ * -1 for unknown ids. */
 FUSE_API int fuse_b200_abi_sizeof(int record);
 /* Number of kernels this library has launched in this process (all entry points). */
 FUSE_API uint64_t fuse_b200_launch_count(void);

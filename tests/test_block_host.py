@@ -148,3 +148,62 @@ def test_torch_arguments_are_refused():
                  lambda: block.rotary(None, None, block.Rotary(128), head_dim=128)):
         with pytest.raises(ValueError):
             call()
+
+
+def attention_params(**kw):
+    p = N.AttentionParams(q=PTR, k=PTR, v=PTR, output=PTR, q_stride=-1, k_stride=-1, v_stride=-1, output_stride=-1, q_rows=256,
+                          kv_rows=512, batch=2, q_len=128, kv_len=256, q_heads=8, kv_heads=2, head_dim=128, causal=1, scale=0.1)
+    for key, value in kw.items():
+        setattr(p, key, value)
+    return p
+
+
+SHAPE_FAULTS = [
+    dict(batch=-1), dict(q_len=-1), dict(kv_len=-1), dict(q_heads=0), dict(kv_heads=0), dict(q_heads=7), dict(window=-1), dict(sinks=-1),
+    dict(causal=0, window=4), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(q_len=129),
+    dict(kv_len=257), dict(q_rows=-1), dict(q_rows=2 ** 31), dict(kv_rows=2 ** 31), dict(q_len=2 ** 30, q_starts=PTR),
+]
+POINTER_FAULTS = [
+    dict(q=None), dict(q=PTR + 8), dict(k=None), dict(v=PTR + 2), dict(output=None), dict(output_stride=1020), dict(q_stride=1028),
+    dict(k_stride=128), dict(v_stride=252), dict(lse=PTR + 2),
+]
+
+
+@pytest.mark.parametrize("bad", SHAPE_FAULTS + POINTER_FAULTS)
+def test_attention_refuses(bad):
+    assert api.launch_attention(attention_params(**bad)) == INVALID
+
+
+@pytest.mark.parametrize("bad", SHAPE_FAULTS)
+def test_attention_workspace_refuses(bad):
+    assert api.attention_workspace_size(attention_params(**bad))[0] == INVALID
+    assert api.attention_backward_workspace_size(N.AttentionBackwardParams(forward=attention_params(**bad)))[0] == INVALID
+
+
+def attention_backward_params(**kw):
+    forward = {key: kw.pop(key) for key in list(kw) if hasattr(N.AttentionParams, key) and key not in ("workspace", "workspace_bytes")}
+    p = N.AttentionBackwardParams(forward=attention_params(**{"lse": PTR, **forward}), grad_output=PTR, grad_q=PTR, grad_k=PTR,
+                                  grad_v=PTR, grad_output_stride=-1, grad_q_stride=-1, grad_k_stride=-1, grad_v_stride=-1,
+                                  workspace=PTR, workspace_bytes=1 << 30)
+    for key, value in kw.items():
+        setattr(p, key, value)
+    return p
+
+
+@pytest.mark.parametrize("bad", SHAPE_FAULTS + POINTER_FAULTS + [
+    dict(lse=None), dict(grad_output=None), dict(grad_q=PTR + 8), dict(grad_k=None), dict(grad_v=None), dict(grad_q_stride=512),
+    dict(grad_k_stride=260), dict(grad_output_stride=8), dict(workspace=None), dict(workspace=PTR + 128), dict(workspace_bytes=8 * 256 * 4 - 1),
+])
+def test_attention_backward_refuses(bad):
+    assert api.launch_attention_backward(attention_backward_params(**bad)) == INVALID
+
+
+def test_attention_without_work_or_support():
+    assert api.launch_attention(attention_params(head_dim=96)) == N.CUDA_ERROR_NOT_SUPPORTED
+    assert api.launch_attention(attention_params(batch=0, q=None)) == 0
+    assert api.launch_attention(attention_params(q_len=0, q=None)) == 0
+    assert api.launch_attention_backward(attention_backward_params(batch=0)) == 0
+    rc, size = api.attention_backward_workspace_size(attention_backward_params())
+    assert rc == 0 and size >= 8 * 256 * 4
+    assert N.lib().fuse_b200_launch_attention(None, None, None) == INVALID
+    assert N.lib().fuse_b200_launch_attention_backward(None, None, None) == INVALID
