@@ -3,7 +3,7 @@
     proj = UlyssesProjections(world, batch=1, seq_local=S, hidden=H, q_heads=32, kv_heads=8, head_dim=128)
     q, k, v = proj.qkv(x, w_qkv)          # x [B*S, H] (this rank's sequence shard) -> this rank's heads,
                                           # every position: [B*S_global, local_heads*d] each
-    a = attention(q, k, v)                # caller's attention, [B*S_global, q_local*d]
+    a = proj.attention(q, k, v, rotary=block.Rotary(128))  # or the caller's attention, [B*S_global, q_local*d]
     y = proj.oproj(a, w_o)                # head->sequence all-to-all + output projection, [B*S, H]
     y.backward(dy)                        # fused backward: dA routed back, dX, dW_qkv, dW_o
 
@@ -32,7 +32,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from . import api
+from . import api, block
 from .world import World
 
 BF16 = torch.bfloat16
@@ -228,6 +228,19 @@ class UlyssesProjections:
         if self.cp > 1:
             self._hook(w_o)
         return _OutputProjection.apply(self, attn, w_o)
+
+    def attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, rotary: block.Rotary | None = None,
+                  causal: bool = True, window: int = 0, sinks: int = 0, scale: float | None = None,
+                  out: torch.Tensor | None = None):
+        """Attention of this rank's heads over every position (block.attention), after rotary positions 0, 1, ... of each
+        sequence when given: what lies between `qkv` and `oproj`.  out: `attention_buffer()`, without gradients."""
+        self._expect(q, (self.rows_global, self.q_local), "q")
+        self._expect(k, (self.rows_global, self.kv_local), "k")
+        self._expect(v, (self.rows_global, self.kv_local), "v")
+        if rotary is not None:
+            q, k = block.rotary(q, k, rotary, head_dim=self.head_dim, seq_len=self.seq_local * self.cp)
+        return block.attention(q, k, v, head_dim=self.head_dim, batch=self.batch, causal=causal, window=window,
+                               sinks=sinks, scale=scale, out=out)
 
     def _expect(self, t: torch.Tensor, shape, name: str) -> None:
         if t.dtype != BF16 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != self.device:
