@@ -53,6 +53,11 @@ struct Args {
   float *partial, *partial_lse;
 };
 
+// What is the same for a whole warp, said so: values that come from memory are not known to be, and the UMMA
+// warp's operands would take the long way through vector registers (measured: 850 cycles for the eight
+// instructions of a 128 x 128 x 128 product that the tensor cores do in 512).
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 struct Sequence {
   int32_t q0, k0;  // first rows
   int32_t ql, kl;  // lengths
@@ -68,12 +73,17 @@ __device__ __forceinline__ void clamp_rows(int64_t start, int32_t length, int32_
   *first = int32_t(start);
   *count = n < 0 ? 0 : int32_t(n);
 }
+// (By whole warps.)
 __device__ __forceinline__ Sequence sequence(const Args& a, int32_t b) {
   Sequence s;
   clamp_rows(a.q_starts ? a.q_starts[b] : int64_t(b) * a.q_len, a.q_lengths ? a.q_lengths[b] : a.q_len, a.q_len, a.q_rows,
              &s.q0, &s.ql);
   clamp_rows(a.kv_starts ? a.kv_starts[b] : int64_t(b) * a.kv_len, a.kv_lengths ? a.kv_lengths[b] : a.kv_len, a.kv_len,
              a.kv_rows, &s.k0, &s.kl);
+  s.q0 = uniform(s.q0);
+  s.k0 = uniform(s.k0);
+  s.ql = uniform(s.ql);
+  s.kl = uniform(s.kl);
   s.off = s.kl - s.ql;
   return s;
 }
@@ -115,10 +125,40 @@ __device__ __forceinline__ bool needs_mask(const Args& a, const Sequence& s, int
   return a.window > 0 && k0 < last - 1 + s.off - a.window + 1 && k0 + kTile > a.sinks;
 }
 
+// The low n of 32 bits (n may be anything).
+__device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// Of the 32 keys from k0 on, those a row sees: keys <= hi that are >= lo or < sinks.
+__device__ __forceinline__ uint32_t visible_keys(int32_t k0, int32_t hi, int32_t lo, int32_t sinks) {
+  return low_bits(hi + 1 - k0) & (~low_bits(lo - k0) | low_bits(sinks - k0));
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two FP32 values in a 64-bit register, for the packed FP32 instructions.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// max(a, b, c), NaN if any is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -127,7 +167,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitContext& w, uint32_t site) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, site));
+  return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, w, site));
 }
 
 // A [128 x kDim] BF16 tile in shared memory: kDim / 64 blocks of 128 rows x 128 bytes, 128-byte swizzle.
@@ -157,25 +197,26 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int32_t row, int32_t va
   ptx::fence_proxy_async_shared();
 }
 
-// D[128 x 128] = A B^T over kDim: both operands K-major tiles (rows of A, rows of B).
+// D[128 x 128] = A B^T over kDim: both operands K-major tiles (rows of A, rows of B).  A converged warp.
 template <int kDim>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile) {
+__device__ __forceinline__ void mma_rows(uint32_t issue, uint32_t d, uint32_t a_tile, uint32_t b_tile) {
   constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kTile, 0, 0);
+  const uint64_t a_desc = ptx::smem_desc_k_sw128(a_tile), b_desc = ptx::smem_desc_k_sw128(b_tile);
 #pragma unroll
   for (uint32_t k = 0; k < kDim / 16; ++k) {
-    const uint32_t at = (k / 4) * TileShape<kDim>::kBlockBytes + (k % 4) * 32;
-    ptx::umma_f16(d, ptx::smem_desc_k_sw128(a_tile + at), ptx::smem_desc_k_sw128(b_tile + at), kIdesc, k != 0 ? 1u : 0u);
+    const uint64_t at = ((k / 4) * TileShape<kDim>::kBlockBytes + (k % 4) * 32) >> 4;
+    ptx::umma_f16_if(issue, d, a_desc + at, b_desc + at, kIdesc, k != 0 ? 1u : 0u);
   }
 }
 // D[128 x kDim] (+)= A[128 x 128] B: A in TMEM (K values 16 k .. 16 k + 15 at column a_column(k)), B a tile whose rows
 // are the K axis.
 template <int kDim, class Column>
-__device__ __forceinline__ void mma_weights(uint32_t d, Column a_column, uint32_t b_tile, bool accumulate) {
+__device__ __forceinline__ void mma_weights(uint32_t issue, uint32_t d, Column a_column, uint32_t b_tile, bool accumulate) {
   constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kDim, 0, 1);
+  const uint64_t b_desc = ptx::smem_desc_mn_sw128(b_tile, TileShape<kDim>::kBlockBytes);
 #pragma unroll
   for (uint32_t k = 0; k < kTile / 16; ++k)
-    ptx::umma_f16_a_tmem(d, a_column(k), ptx::smem_desc_mn_sw128(b_tile + k * 2048u, TileShape<kDim>::kBlockBytes), kIdesc,
-                         accumulate || k != 0 ? 1u : 0u);
+    ptx::umma_f16_a_tmem_if(issue, d, a_column(k), b_desc + uint64_t(k * 128u), kIdesc, k != 0 || accumulate ? 1u : 0u);
 }
 
 template <int kDim>
@@ -200,9 +241,9 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
   using Layout = ForwardLayout<kDim>;
   constexpr int kStages = Layout::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = ptx::smem_u32(smem_raw);
+  const int warp = uniform(int32_t(threadIdx.x >> 5)), lane = threadIdx.x & 31;
 
   // block -> (tokens, head pack, batch, split); the last tokens, which see the most keys, come first
   const int32_t tile_tokens = kTile >> a.pack_shift, packs = a.q_heads >> a.pack_shift;
@@ -263,11 +304,14 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (base - raw) + Layout::kSlot);
+  constexpr uint32_t tmem = 0;  // all 512 columns are this block's
   auto s_tmem = [&](int t) { return tmem + uint32_t(t) * 128u; };
   auto o_tmem = [&](int t) { return tmem + 256u + uint32_t(t) * 128u; };
 
   bool unwound = false;
+  // 168 registers a thread at launch, 64,512 in all: 88 for the first four warps and 208 for the eight
+  // softmax warps are as many
+  if (warp < 4) ptx::setmaxnreg_dec<88>();
   if (warp == 0) {
     if (lane == 0 && it0 < it1) {
       bool ok = true;
@@ -281,101 +325,108 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int s = (it - it0) % kStages;
         const uint32_t phase = ((it - it0) / kStages) & 1;
         const int32_t row = seq.k0 + tiles.tile(it) * kTile;
-        if (!(ok = mbar_wait(k_empty(s), phase ^ 1u, a.wait, kSiteSmemEmpty))) break;
+        if (!(ok = mbar_wait<false>(k_empty(s), phase ^ 1u, a.wait, kSiteSmemEmpty))) break;
         ptx::mbar_expect_tx(k_full(s), Layout::kTileBytes);
         load_tile<kDim>(k_tile(s), &map_k, k_full(s), kv_head, row);
         if (it == it0) load_q(1);
-        if (!(ok = mbar_wait(v_empty(s), phase ^ 1u, a.wait, kSiteSmemEmpty))) break;
+        if (!(ok = mbar_wait<false>(v_empty(s), phase ^ 1u, a.wait, kSiteSmemEmpty))) break;
         ptx::mbar_expect_tx(v_full(s), Layout::kTileBytes);
         load_tile<kDim>(v_tile(s), &map_v, v_full(s), kv_head, row);
       }
       unwound = !ok;
     }
   } else if (warp == 1) {
-    if (lane == 0 && it0 < it1) {
-      bool ok = true, started[2] = {false, false};
+    // the whole warp walks the schedule, one lane issues: the operands of the instructions stay uniform
+    if (it0 < it1) {
+      const uint32_t issue = ptx::elect_one();
+      const KeyRange own0(a, seq, t0, min(t0 + tile_tokens, seq.ql));
+      const KeyRange own1(a, seq, t0 + tile_tokens, min(t0 + 2 * tile_tokens, seq.ql));
+      bool ok = true, started[2] = {false, false}, has_o[2] = {false, false};
       uint32_t p_phase[2] = {0, 0};
-      auto scores = [&](int t, int32_t it) {  // S of tile t; K of `it` has arrived
-        if (!started[t] && !(ok = mbar_wait(q_full(t), 0, a.wait, kSiteSmemFull))) return;
-        mma_rows<kDim>(s_tmem(t), base + t * Layout::kTileBytes, k_tile((it - it0) % kStages));
-        ptx::umma_commit(s_full(t));
-        started[t] = true;
-      };
-      bool has_o[2] = {false, false};
       for (int32_t it = it0 - 1; ok && it < it1; ++it) {
         const bool now = it >= it0, next = it + 1 < it1;
-        const int s = (it - it0) % kStages;
+        const int s = (it - it0) % kStages, s_next = (it + 1 - it0) % kStages;
+        const uint32_t phase = ((it - it0) / kStages) & 1, phase_next = ((it + 1 - it0) / kStages) & 1;
         const int32_t tile = now ? tiles.tile(it) : 0, next_tile = next ? tiles.tile(it + 1) : 0;
         bool have_v = false, have_k = false;
-        for (int t = 0; ok && t < 2; ++t) {
-          if (now && own[t].sees(tile)) {
-            if (!(ok = mbar_wait(p_ready(t), p_phase[t], a.wait, kSiteTmemEmpty))) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const KeyRange& own = t ? own1 : own0;
+          if (ok && now && own.sees(tile)) {
+            ok = warp_wait(p_ready(t), p_phase[t], a.wait, kSiteTmemEmpty);
             p_phase[t] ^= 1u;
-            if (!have_v && !(ok = mbar_wait(v_full(s), ((it - it0) / kStages) & 1, a.wait, kSiteSmemFull))) break;
+            if (ok && !have_v) ok = warp_wait(v_full(s), phase, a.wait, kSiteSmemFull);
             have_v = true;
-            ptx::tc_fence_after();
-            mma_weights<kDim>(o_tmem(t), [&](uint32_t k) { return s_tmem(t) + k * 8u; }, v_tile(s), has_o[t]);
-            has_o[t] = true;
+            if (ok) {
+              ptx::tc_fence_after();
+              mma_weights<kDim>(issue, o_tmem(t), [&](uint32_t k) { return s_tmem(t) + k * 8u; }, v_tile(s), has_o[t]);
+              has_o[t] = true;
+            }
           }
-          if (next && own[t].sees(next_tile)) {
-            if (!have_k && !(ok = mbar_wait(k_full((it + 1 - it0) % kStages), ((it + 1 - it0) / kStages) & 1, a.wait, kSiteSmemFull)))
-              break;
+          if (ok && next && own.sees(next_tile)) {
+            if (!have_k) ok = warp_wait(k_full(s_next), phase_next, a.wait, kSiteSmemFull);
             have_k = true;
-            scores(t, it + 1);
+            if (ok && !started[t]) ok = warp_wait(q_full(t), 0, a.wait, kSiteSmemFull);
+            started[t] = true;
+            if (ok) {
+              mma_rows<kDim>(issue, s_tmem(t), base + t * Layout::kTileBytes, k_tile(s_next));
+              ptx::umma_commit_if(issue, s_full(t));
+            }
           }
         }
-        if (!ok) break;
-        if (now) ptx::umma_commit(v_empty(s));
-        if (next) ptx::umma_commit(k_empty((it + 1 - it0) % kStages));
+        if (ok) {
+          if (now) ptx::umma_commit_if(issue, v_empty(s));
+          if (next) ptx::umma_commit_if(issue, k_empty(s_next));
+        }
       }
-      if (ok) {
-        ptx::umma_commit(o_full);
-      } else {
-        ptx::umma_commit(drain);  // UMMAs already issued retire before TMEM is released
-        mbar_wait(drain, 0u, a.wait, kSiteDrain, false);
-      }
+      ptx::umma_commit_if(issue, ok ? o_full : drain);
+      if (!ok) mbar_wait<false>(drain, 0u, a.wait, kSiteDrain, false);  // UMMAs already issued retire before TMEM is released
       unwound = !ok;
     }
   } else if (warp >= 4) {
+    ptx::setmaxnreg_inc<208>();
     const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const int32_t my_first = t ? t0 + tile_tokens : t0, my_last = min(my_first + tile_tokens, seq.ql);
+    const KeyRange my_range(a, seq, my_first, my_last);
     const uint32_t s_at = s_tmem(t) + lanes, o_at = o_tmem(t) + lanes;
-    const int32_t token = first[t] + (row >> a.pack_shift), head = head0 + (row & (a.pack - 1));
+    const int32_t token = my_first + (row >> a.pack_shift), head = head0 + (row & (a.pack - 1));
     const int32_t pos = token + seq.off;
     const int32_t hi = a.causal ? min(pos, seq.kl - 1) : seq.kl - 1;
     const int32_t lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
     const int32_t sinks = a.window > 0 ? a.sinks : 0;
-    const bool live = first[t] < last[t];
+    const bool live = my_first < my_last;
     float m = -INFINITY, l = 0.0f;  // m: the reference of the exponent, in units of the scaled score's log2
     bool ok = true, begun = false;
     uint32_t phase = 0;
     for (int32_t it = it0; ok && it < it1; ++it) {
       const int32_t tile = tiles.tile(it);
-      if (!own[t].sees(tile)) continue;
+      if (!my_range.sees(tile)) continue;
       if (!(ok = warp_wait(s_full(t), phase, a.wait, kSiteTmemFull))) break;
       ptx::tc_fence_after();
       uint32_t s[4][32];
 #pragma unroll
       for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(s_at + i * 32, s[i]);
       ptx::tmem_wait_ld();
-      if (needs_mask(a, seq, first[t], last[t], tile)) {
-        const int32_t k0 = tile * kTile, h = hi - k0, w = lo - k0, n = sinks - k0;
+      const bool masked = needs_mask(a, seq, my_first, my_last, tile);
+      if (masked) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t seen = visible_keys(tile * kTile + i * 32, hi, lo, sinks);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const int32_t key = i * 32 + c;
-            if (!(key <= h && (key >= w || key < n))) s[i][c] = 0xff800000u;
-          }
+          for (int c = 0; c < 32; ++c) s[i][c] = seen & (1u << c) ? s[i][c] : 0xff800000u;
+        }
       }
       float top[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        top[i] = as_float(s[i][0]);
+        top[i] = max3(as_float(s[i][0]), as_float(s[i][1]), as_float(s[i][2]));
 #pragma unroll
-        for (int c = 1; c < 32; ++c) top[i] = fmaxf(top[i], as_float(s[i][c]));
+        for (int c = 3; c < 31; c += 2) top[i] = max3(top[i], as_float(s[i][c]), as_float(s[i][c + 1]));
+        top[i] = max3(top[i], as_float(s[i][31]), as_float(s[i][31]));
       }
-      const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+      const float largest = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
+      if (largest != largest) l = largest;  // a score that is no number: so is the row
       if (__any_sync(0xffffffffu, largest > m + 8.0f)) {
         const float to = fmaxf(m, largest);
         const float factor = m == -INFINITY ? 0.0f : exp2_approx(m - to);
@@ -397,20 +448,25 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       phase ^= 1u;
       begun = true;
       const float ref = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), ref2 = pair(-ref, -ref);
+      uint64_t sum[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t p[16];
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-          const float x = exp2_approx(fmaf(as_float(s[i][2 * c]), a.scale_log2, -ref));
-          const float y = exp2_approx(fmaf(as_float(s[i][2 * c + 1]), a.scale_log2, -ref));
-          sum[i] += x + y;
+          float x, y;
+          unpair(fma2(pair(as_float(s[i][2 * c]), as_float(s[i][2 * c + 1])), scale2, ref2), x, y);
+          x = exp2_approx(x);
+          y = exp2_approx(y);
+          sum[i] = c ? add2(sum[i], pair(x, y)) : pair(x, y);
           p[c] = pack_bf16(x, y);
         }
         ptx::tmem_st_32x32b_x16(s_at + i * 16, p);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float l0, l1;
+      unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+      l += l0 + l1;
       if (tile * kTile + kTile > seq.kl) {  // values behind the last key (the same for the whole group)
         const int s_v = (it - it0) % kStages;
         if (!(ok = warp_wait(v_full(s_v), ((it - it0) / kStages) & 1, a.wait, kSiteSmemFull))) break;
@@ -425,7 +481,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const bool any = it0 < it1;
       if (any) ok = warp_wait(o_full, 0, a.wait, kSiteTmemFull);
       ptx::tc_fence_after();
-      const bool mine = token < last[t];
+      const bool mine = token < my_last;
       const bool seen = any && l != 0.0f;  // else a row with no visible key (of this split): zeros, -inf
       const float inverse = 1.0f / l;
       const float lse = seen ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;

@@ -70,10 +70,10 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                             const __grid_constant__ BackwardArgs ba) {
   using Layout = QueryGradLayout<kDim>;
   constexpr int kKStages = Layout::kKStages, kVStages = Layout::kVStages;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const Args& a = ba.f;
-  const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = ptx::smem_u32(smem_raw);
+  const int warp = uniform(int32_t(threadIdx.x >> 5)), lane = threadIdx.x & 31;
 
   const int32_t tile_tokens = kTile >> a.pack_shift, packs = a.q_heads >> a.pack_shift;
   int32_t at = int32_t(blockIdx.x);
@@ -130,7 +130,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (base - raw) + Layout::kSlot);
+  constexpr uint32_t tmem = 0;  // all 512 columns are this block's
   const uint32_t s_tmem = tmem, dq_tmem = tmem + 384u;
   auto dp_tmem = [&](uint32_t i) { return tmem + 128u + i * 128u; };
 
@@ -144,49 +144,46 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       for (int32_t it = 0; it < tiles.count; ++it) {
         const uint32_t ks = it % kKStages, vs = it % kVStages;
         const int32_t row = seq.k0 + tiles.tile(it) * kTile;
-        if (!(ok = mbar_wait(k_empty(ks), ((it / kKStages) & 1) ^ 1u, a.wait, kSiteSmemEmpty))) break;
+        if (!(ok = mbar_wait<false>(k_empty(ks), ((it / kKStages) & 1) ^ 1u, a.wait, kSiteSmemEmpty))) break;
         ptx::mbar_expect_tx(k_full(ks), Layout::kTileBytes);
         load_tile<kDim>(k_tile(ks), &map_k, k_full(ks), kv_head, row);
-        if (!(ok = mbar_wait(v_empty(vs), ((it / kVStages) & 1) ^ 1u, a.wait, kSiteSmemEmpty))) break;
+        if (!(ok = mbar_wait<false>(v_empty(vs), ((it / kVStages) & 1) ^ 1u, a.wait, kSiteSmemEmpty))) break;
         ptx::mbar_expect_tx(v_full(vs), Layout::kTileBytes);
         load_tile<kDim>(v_tile(vs), &map_v, v_full(vs), kv_head, row);
       }
       unwound = !ok;
     }
   } else if (warp == 1) {
-    if (lane == 0 && tiles.count > 0) {
-      bool ok = mbar_wait(q_full, 0, a.wait, kSiteSmemFull);
-      auto scores = [&](int32_t it) {  // S and dP of key tile `it`
-        const uint32_t ks = it % kKStages, vs = it % kVStages;
-        if (!(ok = mbar_wait(k_full(ks), (it / kKStages) & 1, a.wait, kSiteSmemFull))) return;
-        ptx::tc_fence_after();
-        mma_rows<kDim>(s_tmem, base + Layout::kQ, k_tile(ks));
-        ptx::umma_commit(s_full);
-        if (!(ok = mbar_wait(v_full(vs), (it / kVStages) & 1, a.wait, kSiteSmemFull))) return;
-        mma_rows<kDim>(dp_tmem(it & 1), base + Layout::kDo, v_tile(vs));
-        ptx::umma_commit(dp_full(it & 1));
-        ptx::umma_commit(v_empty(vs));
-      };
-      if (ok) scores(0);
-      for (int32_t it = 0; ok && it < tiles.count; ++it) {
-        if (it + 1 < tiles.count) {
+    if (tiles.count > 0) {
+      const uint32_t issue = ptx::elect_one();
+      bool ok = warp_wait(q_full, 0, a.wait, kSiteSmemFull);
+      uint32_t ks = 0, k_phase = 0, vs = 0, v_phase = 0, last_ks = 0;
+      for (int32_t it = -1; ok && it < tiles.count; ++it) {
+        if (it + 1 < tiles.count) {  // S and dP of the next key tile
           // S is read into registers, then its columns take the next tile's; dP alternates between two slots,
           // whose dS the product two tiles ago has read
-          if (!(ok = mbar_wait(s_read, it & 1, a.wait, kSiteTmemEmpty))) break;
-          scores(it + 1);
-          if (!ok) break;
+          if (it >= 0 && !(ok = warp_wait(s_read, it & 1, a.wait, kSiteTmemEmpty))) break;
+          if (!(ok = warp_wait(k_full(ks), k_phase, a.wait, kSiteSmemFull))) break;
+          ptx::tc_fence_after();
+          mma_rows<kDim>(issue, s_tmem, base + Layout::kQ, k_tile(ks));
+          ptx::umma_commit_if(issue, s_full);
+          if (!(ok = warp_wait(v_full(vs), v_phase, a.wait, kSiteSmemFull))) break;
+          mma_rows<kDim>(issue, dp_tmem((it + 1) & 1), base + Layout::kDo, v_tile(vs));
+          ptx::umma_commit_if(issue, dp_full((it + 1) & 1));
+          ptx::umma_commit_if(issue, v_empty(vs));
+          if (++vs == kVStages) { vs = 0; v_phase ^= 1u; }
         }
-        if (!(ok = mbar_wait(ds_ready(it & 1), (it >> 1) & 1, a.wait, kSiteTmemEmpty))) break;
-        ptx::tc_fence_after();
-        mma_weights<kDim>(dq_tmem, Halves{dp_tmem(it & 1)}, k_tile(it % kKStages), it > 0);
-        ptx::umma_commit(k_empty(it % kKStages));
+        if (it >= 0) {
+          if (!(ok = warp_wait(ds_ready(it & 1), (it >> 1) & 1, a.wait, kSiteTmemEmpty))) break;
+          ptx::tc_fence_after();
+          mma_weights<kDim>(issue, dq_tmem, Halves{dp_tmem(it & 1)}, k_tile(last_ks), it > 0);
+          ptx::umma_commit_if(issue, k_empty(last_ks));
+        }
+        last_ks = ks;
+        if (++ks == kKStages) { ks = 0; k_phase ^= 1u; }
       }
-      if (ok) {
-        ptx::umma_commit(dq_full);
-      } else {
-        ptx::umma_commit(drain);
-        mbar_wait(drain, 0u, a.wait, kSiteDrain, false);
-      }
+      ptx::umma_commit_if(issue, ok ? dq_full : drain);
+      if (!ok) mbar_wait<false>(drain, 0u, a.wait, kSiteDrain, false);
       unwound = !ok;
     }
   } else if (warp >= 4) {
@@ -211,7 +208,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         }
       }
     }
-    float* parts = reinterpret_cast<float*>(smem_raw + (base - raw) + Layout::kDelta);
+    float* parts = reinterpret_cast<float*>(smem_raw + Layout::kDelta);
     parts[half * kTile + row] = part;
     ptx::named_bar_sync(1, kElementwiseThreads);
     const float delta = parts[row] + parts[kTile + row];
@@ -241,14 +238,12 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       if (lane == 0) ptx::mbar_arrive(s_read);
       const bool masked = needs_mask(a, seq, first, last, tile);
       if (masked) {
-        const int32_t h = hi - k0 - int32_t(columns), w = lo - k0 - int32_t(columns), n = sinks - k0 - int32_t(columns);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t seen = visible_keys(k0 + int32_t(columns) + i * 32, hi, lo, sinks);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const int32_t key = i * 32 + c;
-            if (!(key <= h && (key >= w || key < n))) s[i][c] = 0xff800000u;
-          }
+          for (int c = 0; c < 32; ++c) s[i][c] = seen & (1u << c) ? s[i][c] : 0xff800000u;
+        }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -264,8 +259,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         ptx::tmem_wait_ld();
         if (masked) {  // dP of a key nobody may see can be anything
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (s[i][c] == 0u) dp[c] = __float_as_uint(delta);
+          for (int c = 0; c < 32; ++c) dp[c] = s[i][c] != 0u ? dp[c] : __float_as_uint(delta);
         }
 #pragma unroll
         for (int c = 0; c < 16; ++c)
@@ -349,10 +343,10 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                           const __grid_constant__ BackwardArgs ba) {
   using Layout = KeyGradLayout<kDim>;
   constexpr int kStages = Layout::kStages;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const Args& a = ba.f;
-  const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = ptx::smem_u32(smem_raw);
+  const int warp = uniform(int32_t(threadIdx.x >> 5)), lane = threadIdx.x & 31;
 
   // the first keys, which the most queries see, come first
   const int32_t tile_tokens = kTile >> a.pack_shift;
@@ -377,7 +371,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   auto q_empty = [&](uint32_t s) { return bars + 8u * (11 + kStages + s); };
   auto do_full = [&](uint32_t s) { return bars + 8u * (11 + 2 * kStages + s); };
   auto do_empty = [&](uint32_t s) { return bars + 8u * (11 + 3 * kStages + s); };
-  float* stats = reinterpret_cast<float*>(smem_raw + (base - raw) + Layout::kStats);
+  float* stats = reinterpret_cast<float*>(smem_raw + Layout::kStats);
   auto q_tile = [&](uint32_t s) { return base + Layout::kQ + s * Layout::kTileBytes; };
   auto do_tile = [&](uint32_t s) { return base + Layout::kDo + s * Layout::kTileBytes; };
 
@@ -412,7 +406,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (base - raw) + Layout::kSlot);
+  constexpr uint32_t tmem = 0;  // all 512 columns are this block's
   const uint32_t s_tmem = tmem, dp_tmem = tmem + 128u, dv_tmem = tmem + 256u, dk_tmem = tmem + 384u;
 
   bool unwound = false;
@@ -425,52 +419,50 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       for (int32_t j = 0; j < total; ++j) {
         const uint32_t s = j % kStages, phase = ((j / kStages) & 1) ^ 1u;
         const int32_t row = seq.q0 + first_token(j), head = first_head(j);
-        if (!(ok = mbar_wait(q_empty(s), phase, a.wait, kSiteSmemEmpty))) break;
+        if (!(ok = mbar_wait<false>(q_empty(s), phase, a.wait, kSiteSmemEmpty))) break;
         ptx::mbar_expect_tx(q_full(s), Layout::kTileBytes);
         load_tile<kDim>(q_tile(s), &map_q, q_full(s), head, row);
-        if (!(ok = mbar_wait(do_empty(s), phase, a.wait, kSiteSmemEmpty))) break;
+        if (!(ok = mbar_wait<false>(do_empty(s), phase, a.wait, kSiteSmemEmpty))) break;
         ptx::mbar_expect_tx(do_full(s), Layout::kTileBytes);
         load_tile<kDim>(do_tile(s), &map_do, do_full(s), head, row);
       }
       unwound = !ok;
     }
   } else if (warp == 1) {
-    if (lane == 0 && total > 0) {
+    if (total > 0) {
       // P overwrites S and dS overwrites dP; the UMMAs' issue order keeps each from being overwritten too early
-      bool ok = mbar_wait(kv_full, 0, a.wait, kSiteSmemFull);
-      auto scores = [&](int32_t j) {
-        const uint32_t s = j % kStages;
-        if (!(ok = mbar_wait(q_full(s), (j / kStages) & 1, a.wait, kSiteSmemFull))) return;
-        mma_rows<kDim>(s_tmem, base + Layout::kK, q_tile(s));
-        ptx::umma_commit(s_full);
-      };
-      auto weight_grads = [&](int32_t j) {
-        const uint32_t s = j % kStages;
-        if (!(ok = mbar_wait(do_full(s), (j / kStages) & 1, a.wait, kSiteSmemFull))) return;
-        mma_rows<kDim>(dp_tmem, base + Layout::kV, do_tile(s));
-        ptx::umma_commit(dp_full);
-      };
-      if (ok) scores(0);
-      if (ok) weight_grads(0);
-      for (int32_t j = 0; ok && j < total; ++j) {
-        const uint32_t s = j % kStages;
-        if (!(ok = mbar_wait(p_ready, j & 1, a.wait, kSiteTmemEmpty))) break;
-        ptx::tc_fence_after();
-        mma_weights<kDim>(dv_tmem, Halves{s_tmem}, do_tile(s), j > 0);
-        ptx::umma_commit(do_empty(s));
-        if (j + 1 < total) scores(j + 1);
-        if (!ok || !(ok = mbar_wait(ds_ready, j & 1, a.wait, kSiteTmemEmpty))) break;
-        ptx::tc_fence_after();
-        mma_weights<kDim>(dk_tmem, Halves{dp_tmem}, q_tile(s), j > 0);
-        ptx::umma_commit(q_empty(s));
-        if (j + 1 < total) weight_grads(j + 1);
+      const uint32_t issue = ptx::elect_one();
+      bool ok = warp_wait(kv_full, 0, a.wait, kSiteSmemFull);
+      uint32_t s = 0, s_next = 0, phase = 0;  // stages of tiles j and j + 1, phase of the latter
+      for (int32_t j = -1; ok && j < total; ++j) {
+        const bool now = j >= 0, next = j + 1 < total;
+        if (now) {
+          if (!(ok = warp_wait(p_ready, j & 1, a.wait, kSiteTmemEmpty))) break;
+          ptx::tc_fence_after();
+          mma_weights<kDim>(issue, dv_tmem, Halves{s_tmem}, do_tile(s), j > 0);
+          ptx::umma_commit_if(issue, do_empty(s));
+        }
+        if (next) {
+          if (!(ok = warp_wait(q_full(s_next), phase, a.wait, kSiteSmemFull))) break;
+          mma_rows<kDim>(issue, s_tmem, base + Layout::kK, q_tile(s_next));
+          ptx::umma_commit_if(issue, s_full);
+        }
+        if (now) {
+          if (!(ok = warp_wait(ds_ready, j & 1, a.wait, kSiteTmemEmpty))) break;
+          ptx::tc_fence_after();
+          mma_weights<kDim>(issue, dk_tmem, Halves{dp_tmem}, q_tile(s), j > 0);
+          ptx::umma_commit_if(issue, q_empty(s));
+        }
+        if (next) {
+          if (!(ok = warp_wait(do_full(s_next), phase, a.wait, kSiteSmemFull))) break;
+          mma_rows<kDim>(issue, dp_tmem, base + Layout::kV, do_tile(s_next));
+          ptx::umma_commit_if(issue, dp_full);
+        }
+        s = s_next;
+        if (++s_next == kStages) { s_next = 0; phase ^= 1u; }
       }
-      if (ok) {
-        ptx::umma_commit(grads_full);
-      } else {
-        ptx::umma_commit(drain);
-        mbar_wait(drain, 0u, a.wait, kSiteDrain, false);
-      }
+      ptx::umma_commit_if(issue, ok ? grads_full : drain);
+      if (!ok) mbar_wait<false>(drain, 0u, a.wait, kSiteDrain, false);
       unwound = !ok;
     }
   } else if (warp == 3) {
@@ -536,13 +528,15 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
       }
       if (masked) {
-        // columns [low, high) of this half; far bounds stay within 31 bits
-        const int64_t low = (int64_t(from) - t0) * a.pack - columns, high = (int64_t(to) - t0) * a.pack - columns;
+        // the columns of tokens [from, to): those in [low, high)
+        const int32_t low = (max(from, t0) - t0) << a.pack_shift, high = (min(to, t0 + tile_tokens) - t0) * a.pack;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+          const int32_t at = int32_t(columns) + i * 32;
+          const uint32_t seen = low_bits(high - at) & ~low_bits(low - at);
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (i * 32 + c < low || i * 32 + c >= high) p[i][c] = 0u;
+          for (int c = 0; c < 32; ++c) p[i][c] = seen & (1u << c) ? p[i][c] : 0u;
+        }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -578,8 +572,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (p[i][c] == 0u) dp[c] = 0u;
+          for (int c = 0; c < 32; ++c) dp[c] = p[i][c] != 0u ? dp[c] : 0u;
         }
 #pragma unroll
         for (int c = 0; c < 16; ++c)

@@ -57,8 +57,8 @@ __device__ __forceinline__ bool aborted(const WaitContext& w) {
   return ptx::ld_relaxed_gpu(w.status) == w.launch_id;
 }
 
-__device__ __noinline__ inline void report_timeout(const WaitContext w, uint32_t code, uint32_t site,
-                                            uint32_t index, uint32_t observed, uint32_t expected) {
+__device__ __forceinline__ void write_timeout(const WaitContext& w, uint32_t code, uint32_t site, uint32_t index,
+                                              uint32_t observed, uint32_t expected) {
   // The record goes to the first waiter of THIS launch: a record that an earlier launch left
   // uncleared is overwritten, so that the abort fan-out below still works.
   uint32_t owner = ptx::ld_relaxed_gpu(w.status);
@@ -83,9 +83,16 @@ __device__ __noinline__ inline void report_timeout(const WaitContext w, uint32_t
   }
 }
 
+__device__ __noinline__ inline void report_timeout(const WaitContext w, uint32_t code, uint32_t site,
+                                            uint32_t index, uint32_t observed, uint32_t expected) {
+  write_timeout(w, code, site, index, observed, expected);
+}
+
 // Waits for the mbarrier phase with the given parity.  With `honor_abort` the wait also ends
 // when another waiter of this launch has given up; the drains that run while unwinding pass
 // false so that copies and UMMAs in flight still get their (bounded) time to land.
+// kCall: the report is a call.  Kernels that change their register count (setmaxnreg) hold no calls.
+template <bool kCall = true>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const WaitContext& w,
                                           uint32_t site, bool honor_abort = true) {
   if (ptx::mbar_try_wait(bar, parity)) return true;
@@ -95,7 +102,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
     if ((spin & 31u) == 0u) {
       if (honor_abort && aborted(w)) return false;
       if (ptx::globaltimer() - start > w.budget_ns) {
-        report_timeout(w, kStatusMbarrierTimeout, site, bar, parity, 0);
+        if constexpr (kCall) report_timeout(w, kStatusMbarrierTimeout, site, bar, parity, 0);
+        else write_timeout(w, kStatusMbarrierTimeout, site, bar, parity, 0);
         return false;
       }
     }
