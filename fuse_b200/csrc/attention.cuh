@@ -11,15 +11,14 @@
 // the tensor map's box brings them in that order.  A group of heads then reads each key tile once, and a few
 // new tokens of many heads still fill rows.
 //
-// Roles (12 warps): warp 0 loads (TMA: both Q tiles, then K and V tiles through two rings), warp 1 issues the
-// UMMAs, warp 2 allocates TMEM, warps 4-7 and 8-11 are one softmax group per tile, one thread per row.
+// Roles (12 warps): warp 0 loads (TMA: both Q tiles, then K and V tiles through two rings), warps 1 and 3 issue the
+// UMMAs of one tile each, warp 2 allocates TMEM, warps 4-7 and 8-11 are one softmax group per tile, one thread per row.
 // TMEM (512 columns): S of either tile (128 FP32 columns each; P overwrites the first 64 of its own S as
 // packed BF16 and is the A operand of P V straight from there) and O of either tile.
 //
-// The UMMA order is P V of tile 0, S of tile 0 for the next keys, then the same for tile 1: while one tile's
-// softmax runs, the tensor cores work for the other.  The UMMAs of a CTA execute in issue order, so S may
-// overwrite the P that the UMMA before it reads, and "S of the next keys is complete" implies "O holds all
-// keys before", which is what a softmax group needs to rescale O in place.
+// The UMMAs of a tile are issued in the order P V, S of the next keys: while one tile's softmax runs, the tensor cores
+// work for the other.  They execute in issue order, so S may overwrite the P that the UMMA before it reads, and "S of
+// the next keys is complete" implies "O holds all keys before", which is what a softmax group needs to rescale O in place.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then
 // stay below 2^8 in BF16 and the sums below 2^8 kv_len in FP32; the result is divided by the same sum, so
@@ -101,9 +100,8 @@ struct KeyRange {
     if (first >= last || end < 0) end = 0;
     sinks = a.window > 0 && a.sinks > 0 ? (a.sinks < end ? a.sinks : end) : 0;
   }
-  __device__ __forceinline__ bool sees(int32_t tile) const {
-    return tile * kTile < end && ((tile + 1) * kTile > lo || tile * kTile < sinks);
-  }
+  // Whether any of the `keys` keys from k0 on is seen.
+  __device__ __forceinline__ bool sees(int32_t k0, int32_t keys) const { return k0 < end && (k0 + keys > lo || k0 < sinks); }
 };
 // Tiles of a range in the order they are visited.
 struct TileList {
@@ -116,13 +114,13 @@ struct TileList {
   }
   __device__ __forceinline__ int32_t tile(int32_t i) const { return i < sink_tiles ? i : first + i - sink_tiles; }
 };
-// Whether some row among tokens [first, last) does not see all of a key tile.
-__device__ __forceinline__ bool needs_mask(const Args& a, const Sequence& s, int32_t first, int32_t last, int32_t tile) {
-  const int32_t k0 = tile * kTile;
-  if (k0 + kTile > s.kl) return true;
+// Whether some row among tokens [first, last) does not see all of the `keys` keys from k0 on.
+__device__ __forceinline__ bool needs_mask(const Args& a, const Sequence& s, int32_t first, int32_t last, int32_t k0,
+                                           int32_t keys) {
+  if (k0 + keys > s.kl) return true;
   if (!a.causal) return false;
-  if (k0 + kTile - 1 > first + s.off) return true;
-  return a.window > 0 && k0 < last - 1 + s.off - a.window + 1 && k0 + kTile > a.sinks;
+  if (k0 + keys - 1 > first + s.off) return true;
+  return a.window > 0 && k0 < last - 1 + s.off - a.window + 1 && k0 + keys > a.sinks;
 }
 
 // The low n of 32 bits (n may be anything).
@@ -166,8 +164,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
+// A whole warp waits together (the common case, a barrier that is through or about to be, is one vote).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitContext& w, uint32_t site) {
-  return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, w, site));
+  if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+  const uint64_t start = ptx::globaltimer();
+  for (uint32_t spin = 1;; ++spin) {
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+    if ((spin & 31u) == 0u) {
+      bool over = aborted(w);
+      if (!over && ptx::globaltimer() - start > w.budget_ns) {
+        write_timeout(w, kStatusMbarrierTimeout, site, bar, parity, 0);
+        over = true;
+      }
+      if (__any_sync(0xffffffffu, over)) return false;
+    }
+  }
 }
 
 // A [128 x kDim] BF16 tile in shared memory: kDim / 64 blocks of 128 rows x 128 bytes, 128-byte swizzle.
@@ -197,10 +208,11 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int32_t row, int32_t va
   ptx::fence_proxy_async_shared();
 }
 
-// D[128 x 128] = A B^T over kDim: both operands K-major tiles (rows of A, rows of B).  A converged warp.
-template <int kDim>
+// D[128 x kColumns] = A B^T over kDim: both operands K-major tiles, of B the kColumns rows from `b_tile` on.
+// A converged warp.
+template <int kDim, int kColumns = kTile>
 __device__ __forceinline__ void mma_rows(uint32_t issue, uint32_t d, uint32_t a_tile, uint32_t b_tile) {
-  constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kTile, 0, 0);
+  constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kColumns, 0, 0);
   const uint64_t a_desc = ptx::smem_desc_k_sw128(a_tile), b_desc = ptx::smem_desc_k_sw128(b_tile);
 #pragma unroll
   for (uint32_t k = 0; k < kDim / 16; ++k) {
@@ -208,16 +220,22 @@ __device__ __forceinline__ void mma_rows(uint32_t issue, uint32_t d, uint32_t a_
     ptx::umma_f16_if(issue, d, a_desc + at, b_desc + at, kIdesc, k != 0 ? 1u : 0u);
   }
 }
-// D[128 x kDim] (+)= A[128 x 128] B: A in TMEM (K values 16 k .. 16 k + 15 at column a_column(k)), B a tile whose rows
-// are the K axis.
-template <int kDim, class Column>
+// D[128 x kDim] (+)= A[128 x kRows] B: A in TMEM (K values 16 k .. 16 k + 15 at column a_column(k)), B the kRows rows of
+// a tile from `b_tile` on, which are the K axis.
+template <int kDim, int kRows = kTile, class Column>
 __device__ __forceinline__ void mma_weights(uint32_t issue, uint32_t d, Column a_column, uint32_t b_tile, bool accumulate) {
   constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kDim, 0, 1);
   const uint64_t b_desc = ptx::smem_desc_mn_sw128(b_tile, TileShape<kDim>::kBlockBytes);
 #pragma unroll
-  for (uint32_t k = 0; k < kTile / 16; ++k)
+  for (uint32_t k = 0; k < kRows / 16; ++k)
     ptx::umma_f16_a_tmem_if(issue, d, a_column(k), b_desc + uint64_t(k * 128u), kIdesc, k != 0 || accumulate ? 1u : 0u);
 }
+
+// An operand in TMEM whose K values lie in consecutive columns.
+struct Columns {
+  uint32_t base;
+  __device__ __forceinline__ uint32_t operator()(uint32_t k) const { return base + k * 8u; }
+};
 
 template <int kDim>
 struct ForwardLayout {
@@ -226,10 +244,10 @@ struct ForwardLayout {
   static constexpr uint32_t kK = 2 * kTileBytes;
   static constexpr uint32_t kV = kK + kStages * kTileBytes;
   static constexpr uint32_t kBarriers = kV + kStages * kTileBytes;
-  // q_full[2], s_full[2], p_ready[2], o_full, drain, then k_full, k_empty, v_full, v_empty [kStages]
-  static constexpr uint32_t kNumBarriers = 8 + 4 * kStages;
+  // q_full[2], s_full[2], p_ready[2], drain[2], o_full, then k_full, k_empty, v_full, v_empty [kStages]
+  static constexpr uint32_t kNumBarriers = 9 + 4 * kStages;
   static constexpr uint32_t kSlot = kBarriers + kNumBarriers * 8;
-  static constexpr uint32_t kDynamicBytes = kSlot + 16 + 1024;
+  static constexpr uint32_t kDynamicBytes = kSlot + 16;
   static_assert(kDynamicBytes <= 227 * 1024, "shared memory budget");
   static_assert(kDynamicBytes > 114 * 1024, "must force one CTA per SM (all of TMEM is allocated)");
 };
@@ -261,7 +279,6 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int32_t first[2] = {t0, t0 + tile_tokens};
   const int32_t last[2] = {min(t0 + tile_tokens, seq.ql), min(t0 + 2 * tile_tokens, seq.ql)};
   const KeyRange range(a, seq, t0, last[1]);
-  const KeyRange own[2] = {KeyRange(a, seq, first[0], last[0]), KeyRange(a, seq, first[1], last[1])};
   const TileList tiles(range);
   const int32_t per_split = (tiles.count + a.splits - 1) / a.splits;
   const int32_t it0 = min(split * per_split, tiles.count), it1 = min(it0 + per_split, tiles.count);
@@ -270,11 +287,12 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   auto q_full = [&](int t) { return bars + 8u * t; };
   auto s_full = [&](int t) { return bars + 8u * (2 + t); };
   auto p_ready = [&](int t) { return bars + 8u * (4 + t); };
-  const uint32_t o_full = bars + 8u * 6, drain = bars + 8u * 7;
-  auto k_full = [&](int s) { return bars + 8u * (8 + s); };
-  auto k_empty = [&](int s) { return bars + 8u * (8 + kStages + s); };
-  auto v_full = [&](int s) { return bars + 8u * (8 + 2 * kStages + s); };
-  auto v_empty = [&](int s) { return bars + 8u * (8 + 3 * kStages + s); };
+  auto drain = [&](int t) { return bars + 8u * (6 + t); };
+  const uint32_t o_full = bars + 8u * 8;
+  auto k_full = [&](int s) { return bars + 8u * (9 + s); };
+  auto k_empty = [&](int s) { return bars + 8u * (9 + kStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (9 + 2 * kStages + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (9 + 3 * kStages + s); };
   auto k_tile = [&](int s) { return base + Layout::kK + s * Layout::kTileBytes; };
   auto v_tile = [&](int s) { return base + Layout::kV + s * Layout::kTileBytes; };
 
@@ -285,15 +303,15 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(q_full(t), 1);
       ptx::mbar_init(s_full(t), 1);
+      ptx::mbar_init(drain(t), 1);
       ptx::mbar_init(p_ready(t), 4);  // one arrival per warp of the softmax group
     }
-    ptx::mbar_init(o_full, 1);
-    ptx::mbar_init(drain, 1);
+    ptx::mbar_init(o_full, 2);  // from here on 2: a commit of either issuing warp
     for (int s = 0; s < kStages; ++s) {
       ptx::mbar_init(k_full(s), 1);
-      ptx::mbar_init(k_empty(s), 1);
+      ptx::mbar_init(k_empty(s), 2);
       ptx::mbar_init(v_full(s), 1);
-      ptx::mbar_init(v_empty(s), 1);
+      ptx::mbar_init(v_empty(s), 2);
     }
     ptx::fence_mbar_init();
   }
@@ -309,8 +327,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   auto o_tmem = [&](int t) { return tmem + 256u + uint32_t(t) * 128u; };
 
   bool unwound = false;
-  // 168 registers a thread at launch, 64,512 in all: 88 for the first four warps and 208 for the eight
-  // softmax warps are as many
+  // 168 registers a thread at launch, 64,512 in all: 88 for the first four warps and 208 for the eight softmax warps
+  // are as many
   if (warp < 4) ptx::setmaxnreg_dec<88>();
   if (warp == 0) {
     if (lane == 0 && it0 < it1) {
@@ -335,52 +353,45 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       unwound = !ok;
     }
-  } else if (warp == 1) {
-    // the whole warp walks the schedule, one lane issues: the operands of the instructions stay uniform
+  } else if (warp == 1 || warp == 3) {
+    // One warp per tile, on two quarters of the SM: beside the softmax warps a warp gets an instruction through every
+    // ten cycles or so, and the waits and commits of both tiles would be more than one warp's time.  The whole warp walks
+    // the schedule and one lane issues: the operands of the instructions stay uniform.
+    const int t = warp >> 1;
     if (it0 < it1) {
       const uint32_t issue = ptx::elect_one();
-      const KeyRange own0(a, seq, t0, min(t0 + tile_tokens, seq.ql));
-      const KeyRange own1(a, seq, t0 + tile_tokens, min(t0 + 2 * tile_tokens, seq.ql));
-      bool ok = true, started[2] = {false, false}, has_o[2] = {false, false};
-      uint32_t p_phase[2] = {0, 0};
+      const int32_t my_first = t0 + t * tile_tokens;
+      const KeyRange own(a, seq, my_first, min(my_first + tile_tokens, seq.ql));
+      const uint32_t q_tile = base + t * Layout::kTileBytes;
+      auto seen = [&](int32_t it) { return it < it1 && own.sees(tiles.tile(it) * kTile, kTile); };
+      bool ok = my_first >= seq.ql || warp_wait(q_full(t), 0, a.wait, kSiteSmemFull);
+      uint32_t p_phase = 0, has_o = 0;
+      uint32_t s = 0, s_next = 0, v_phase = 0, k_phase = 0;  // stages of V of tile `it` and of K of tile it + 1
+      bool now = false, next = seen(it0);
       for (int32_t it = it0 - 1; ok && it < it1; ++it) {
-        const bool now = it >= it0, next = it + 1 < it1;
-        const int s = (it - it0) % kStages, s_next = (it + 1 - it0) % kStages;
-        const uint32_t phase = ((it - it0) / kStages) & 1, phase_next = ((it + 1 - it0) / kStages) & 1;
-        const int32_t tile = now ? tiles.tile(it) : 0, next_tile = next ? tiles.tile(it + 1) : 0;
-        bool have_v = false, have_k = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const KeyRange& own = t ? own1 : own0;
-          if (ok && now && own.sees(tile)) {
-            ok = warp_wait(p_ready(t), p_phase[t], a.wait, kSiteTmemEmpty);
-            p_phase[t] ^= 1u;
-            if (ok && !have_v) ok = warp_wait(v_full(s), phase, a.wait, kSiteSmemFull);
-            have_v = true;
-            if (ok) {
-              ptx::tc_fence_after();
-              mma_weights<kDim>(issue, o_tmem(t), [&](uint32_t k) { return s_tmem(t) + k * 8u; }, v_tile(s), has_o[t]);
-              has_o[t] = true;
-            }
-          }
-          if (ok && next && own.sees(next_tile)) {
-            if (!have_k) ok = warp_wait(k_full(s_next), phase_next, a.wait, kSiteSmemFull);
-            have_k = true;
-            if (ok && !started[t]) ok = warp_wait(q_full(t), 0, a.wait, kSiteSmemFull);
-            started[t] = true;
-            if (ok) {
-              mma_rows<kDim>(issue, s_tmem(t), base + t * Layout::kTileBytes, k_tile(s_next));
-              ptx::umma_commit_if(issue, s_full(t));
-            }
-          }
+        if (it + 1 < it1 && !(ok = warp_wait(k_full(s_next), k_phase, a.wait, kSiteSmemFull))) break;
+        if (it >= it0 && !(ok = warp_wait(v_full(s), v_phase, a.wait, kSiteSmemFull))) break;
+        if (now) {
+          if (!(ok = warp_wait(p_ready(t), p_phase, a.wait, kSiteTmemEmpty))) break;
+          ptx::tc_fence_after();
+          mma_weights<kDim>(issue, o_tmem(t), Columns{s_tmem(t)}, v_tile(s), has_o);
+          has_o = 1;
+          p_phase ^= 1u;
         }
-        if (ok) {
-          if (now) ptx::umma_commit_if(issue, v_empty(s));
-          if (next) ptx::umma_commit_if(issue, k_empty(s_next));
+        if (next) {
+          mma_rows<kDim>(issue, s_tmem(t), q_tile, k_tile(s_next));
+          ptx::umma_commit_if(issue, s_full(t));
         }
+        if (it >= it0) ptx::umma_commit_if(issue, v_empty(s));
+        if (it + 1 < it1) ptx::umma_commit_if(issue, k_empty(s_next));
+        now = next;
+        next = seen(it + 2);
+        s = s_next;
+        v_phase = k_phase;
+        if (++s_next == kStages) { s_next = 0; k_phase ^= 1u; }
       }
-      ptx::umma_commit_if(issue, ok ? o_full : drain);
-      if (!ok) mbar_wait<false>(drain, 0u, a.wait, kSiteDrain, false);  // UMMAs already issued retire before TMEM is released
+      ptx::umma_commit_if(issue, ok ? o_full : drain(t));
+      if (!ok) mbar_wait<false>(drain(t), 0u, a.wait, kSiteDrain, false);  // UMMAs already issued retire before TMEM is released
       unwound = !ok;
     }
   } else if (warp >= 4) {
@@ -389,30 +400,31 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const int32_t my_first = t ? t0 + tile_tokens : t0, my_last = min(my_first + tile_tokens, seq.ql);
     const KeyRange my_range(a, seq, my_first, my_last);
-    const uint32_t s_at = s_tmem(t) + lanes, o_at = o_tmem(t) + lanes;
+    const uint32_t o_at = o_tmem(t) + lanes;
     const int32_t token = my_first + (row >> a.pack_shift), head = head0 + (row & (a.pack - 1));
     const int32_t pos = token + seq.off;
     const int32_t hi = a.causal ? min(pos, seq.kl - 1) : seq.kl - 1;
     const int32_t lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
     const int32_t sinks = a.window > 0 ? a.sinks : 0;
     const bool live = my_first < my_last;
+    const uint32_t s_at = s_tmem(t) + lanes;
     float m = -INFINITY, l = 0.0f;  // m: the reference of the exponent, in units of the scaled score's log2
     bool ok = true, begun = false;
     uint32_t phase = 0;
     for (int32_t it = it0; ok && it < it1; ++it) {
-      const int32_t tile = tiles.tile(it);
-      if (!my_range.sees(tile)) continue;
+      const int32_t k0 = tiles.tile(it) * kTile;
+      if (!my_range.sees(k0, kTile)) continue;
       if (!(ok = warp_wait(s_full(t), phase, a.wait, kSiteTmemFull))) break;
+      phase ^= 1u;
       ptx::tc_fence_after();
       uint32_t s[4][32];
 #pragma unroll
       for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(s_at + i * 32, s[i]);
       ptx::tmem_wait_ld();
-      const bool masked = needs_mask(a, seq, my_first, my_last, tile);
-      if (masked) {
+      if (needs_mask(a, seq, my_first, my_last, k0, kTile)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t seen = visible_keys(tile * kTile + i * 32, hi, lo, sinks);
+          const uint32_t seen = visible_keys(k0 + i * 32, hi, lo, sinks);
 #pragma unroll
           for (int c = 0; c < 32; ++c) s[i][c] = seen & (1u << c) ? s[i][c] : 0xff800000u;
         }
@@ -445,10 +457,15 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
         }
       }
-      phase ^= 1u;
       begun = true;
       const float ref = m == -INFINITY ? 0.0f : m;
       const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), ref2 = pair(-ref, -ref);
+      const int valid = seq.kl - k0;
+      if (valid < kTile) {  // values behind the last key (the same for the whole group)
+        const int s_v = (it - it0) % kStages;
+        if (!(ok = warp_wait(v_full(s_v), ((it - it0) / kStages) & 1, a.wait, kSiteSmemFull))) break;
+        zero_rows<kDim>(v_tile(s_v), row, valid);
+      }
       uint64_t sum[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -464,18 +481,13 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         ptx::tmem_st_32x32b_x16(s_at + i * 16, p);
       }
-      float l0, l1;
-      unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
-      l += l0 + l1;
-      if (tile * kTile + kTile > seq.kl) {  // values behind the last key (the same for the whole group)
-        const int s_v = (it - it0) % kStages;
-        if (!(ok = warp_wait(v_full(s_v), ((it - it0) / kStages) & 1, a.wait, kSiteSmemFull))) break;
-        zero_rows<kDim>(v_tile(s_v), row, seq.kl - tile * kTile);
-      }
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(p_ready(t));
+      float l0, l1;
+      unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+      l += l0 + l1;
     }
     if (ok && live) {
       const bool any = it0 < it1;

@@ -236,7 +236,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(s_read);
-      const bool masked = needs_mask(a, seq, first, last, tile);
+      const bool masked = needs_mask(a, seq, first, last, k0, kTile);
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
