@@ -154,12 +154,49 @@ cudaError_t attention(const fuse_b200_attention_params& p, const fuse_b200_optio
                            : launch_forward<64>(p, a, q_stride, k_stride, v_stride, stream);
 }
 
-size_t delta_bytes(const fuse_b200_attention_params& p) { return size_t(p.q_heads) * size_t(p.q_rows) * sizeof(float); }
+size_t delta_bytes(const fuse_b200_attention_params& p) {
+  return (size_t(p.q_heads) * size_t(p.q_rows) * sizeof(float) + 255) & ~size_t{255};
+}
+
+// Query tiles that one block of the key gradients takes at most.  Key tiles see very unequal numbers of them (the first
+// key of a causal sequence all, the last one; a sink all, any other key a window's), and with few KV heads there
+// are fewer key tiles than SMs.  About two blocks per SM of equal size (measured: 450 us for a backward of 8192 x 8 / 2 heads, 478 with three, 502 with six), as every
+// further block costs its FP32 partial sums (128 KiB written and read with heads of 128); shorter than eight
+// tiles, a block's set-up shows.
+struct ChunkPlan {
+  int32_t chunk, max_chunks, key_tiles;
+  size_t partial_bytes;
+};
+ChunkPlan plan_chunks(const fuse_b200_attention_params& p, int sm_count) {
+  const int32_t pack = packed_heads(p), tokens = attn::kTile / pack, packs = p.q_heads / p.kv_heads / pack;
+  ChunkPlan plan{};
+  plan.key_tiles = (p.kv_len + attn::kTile - 1) / attn::kTile;
+  const int64_t longest = int64_t((p.q_len + tokens - 1) / tokens) * packs;  // every query tile
+  double seen = double(longest);
+  if (p.causal && p.window > 0 && p.window < p.kv_len) {
+    const double window = double((int64_t(p.window) + attn::kTile) / tokens + 1) * packs;
+    if (window < seen) seen = window;
+  } else if (p.causal && p.kv_len < 2 * int64_t(p.q_len)) {
+    seen *= 0.5;  // (of the keys that are queries' own; those before are seen by all)
+  }
+  const double total = seen * plan.key_tiles * p.kv_heads * p.batch;
+  int64_t chunk = int64_t(std::ceil(total / (2.0 * sm_count)));
+  if (chunk < 8) chunk = 8;
+  if (chunk > longest) chunk = longest > 0 ? longest : 1;
+  plan.chunk = int32_t(chunk);
+  plan.max_chunks = int32_t((longest + chunk - 1) / chunk);
+  if (plan.max_chunks < 1) plan.max_chunks = 1;
+  if (plan.max_chunks > 1)
+    plan.partial_bytes = size_t(plan.key_tiles) * p.kv_heads * p.batch * plan.max_chunks * 2 * attn::kTile * p.head_dim * sizeof(float);
+  return plan;
+}
 
 cudaError_t backward_workspace_size(const fuse_b200_attention_backward_params& p, size_t* bytes) {
-  const cudaError_t status = check_shape(p.forward);
+  cudaError_t status = check_shape(p.forward);
   if (status != cudaSuccess) return status;
-  *bytes = delta_bytes(p.forward);
+  DeviceInfo info;
+  if ((status = launch::check_device(&info)) != cudaSuccess) return status;
+  *bytes = delta_bytes(p.forward) + plan_chunks(p.forward, info.sm_count).partial_bytes;
   return cudaSuccess;
 }
 
@@ -183,15 +220,19 @@ cudaError_t launch_backward(const fuse_b200_attention_params& p, const attn::Bac
                                               attn::kTile, 1)) != cudaSuccess)
     return status;
   const int64_t query_tiles = (int64_t(p.q_len) + tokens - 1) / tokens * (p.q_heads / a.pack) * p.batch;
-  const int64_t key_tiles = (int64_t(p.kv_len) + attn::kTile - 1) / attn::kTile * p.kv_heads * p.batch;
-  if (query_tiles > INT32_MAX || key_tiles > INT32_MAX) return cudaErrorInvalidValue;
+  const int64_t key_tiles = int64_t(b.key_tiles) * p.kv_heads * p.batch, key_blocks = key_tiles * b.max_chunks;
+  if (query_tiles > INT32_MAX || key_blocks > INT32_MAX) return cudaErrorInvalidValue;
   if (query_tiles > 0 &&
       (status = host::launch_kernel(attn::attention_query_grad_kernel<kDim>, int(query_tiles), attn::kBackwardThreads,
                                     attn::QueryGradLayout<kDim>::kDynamicBytes, false, stream, q, d_o, k, v, b)) != cudaSuccess)
     return status;
-  if (key_tiles > 0)
-    status = host::launch_kernel(attn::attention_key_grad_kernel<kDim>, int(key_tiles), attn::kBackwardThreads,
-                                 attn::KeyGradLayout<kDim>::kDynamicBytes, false, stream, q, d_o, k, v, b);
+  if (key_tiles == 0) return cudaSuccess;
+  status = host::launch_kernel(attn::attention_key_grad_kernel<kDim>, int(key_blocks), attn::kBackwardThreads,
+                               attn::KeyGradLayout<kDim>::kDynamicBytes, false, stream, q, d_o, k, v, b);
+  if (status != cudaSuccess || b.max_chunks == 1) return status;
+  attn::attention_key_grad_join_kernel<kDim><<<dim3(unsigned(key_tiles), key_tiles < 592 ? 8 : 2), 256, 0, stream>>>(b);
+  status = cudaGetLastError();
+  if (status == cudaSuccess) host::count_launch();
   return status;
 }
 
@@ -221,6 +262,12 @@ cudaError_t attention_backward(const fuse_b200_attention_backward_params& g, con
     return cudaErrorInvalidValue;
   DeviceInfo info;
   if ((status = launch::check_device(&info)) != cudaSuccess) return status;
+  const ChunkPlan plan = plan_chunks(p, info.sm_count);
+  if (g.workspace_bytes < delta_bytes(p) + plan.partial_bytes) return cudaErrorInvalidValue;
+  b.chunk = plan.chunk;
+  b.max_chunks = plan.max_chunks;
+  b.key_tiles = plan.key_tiles;
+  b.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(g.workspace) + delta_bytes(p));
   b.o = p.output;
   b.d_o = g.grad_output;
   b.lse = p.lse;

@@ -27,6 +27,9 @@ struct BackwardArgs {
   float* delta;  // [q_heads][q_rows]
   uint16_t *dq, *dk, *dv;
   int64_t dq_stride, dk_stride, dv_stride;
+  // the key gradients of a key tile that more than `chunk` query tiles see are made by several blocks
+  int32_t chunk, max_chunks, key_tiles;
+  float* partial;  // [batch][kv head][key tile][max_chunks][dV, dK][128][head_dim]
 };
 
 constexpr int kBackwardThreads = 384, kElementwiseThreads = 256;
@@ -223,6 +226,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const int32_t hi = a.causal ? min(pos, seq.kl - 1) : seq.kl - 1;
     const int32_t lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
     const int32_t sinks = a.window > 0 ? a.sinks : 0;
+    const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), minus_lse = pair(-lse, -lse), minus_delta = pair(-delta, -delta);
     bool ok = true;
     for (int32_t it = 0; it < tiles.count; ++it) {
       const int32_t tile = tiles.tile(it), k0 = tile * kTile;
@@ -248,7 +252,12 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int c = 0; c < 32; ++c) s[i][c] = __float_as_uint(exp2_approx(fmaf(as_float(s[i][c]), a.scale_log2, -lse)));
+        for (int c = 0; c < 32; c += 2) {
+          float x, y;
+          unpair(fma2(pair(as_float(s[i][c]), as_float(s[i][c + 1])), scale2, minus_lse), x, y);
+          s[i][c] = __float_as_uint(exp2_approx(x));
+          s[i][c + 1] = __float_as_uint(exp2_approx(y));
+        }
       if (k0 + kTile > seq.kl && half == 0) zero_rows<kDim>(k_tile(it % kKStages), row, seq.kl - k0);  // S has read it
       if (!(ok = warp_wait(dp_full(slot), (it >> 1) & 1, a.wait, kSiteTmemFull))) break;
       ptx::tc_fence_after();
@@ -263,8 +272,8 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         }
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          ds[c] = pack_bf16(as_float(s[i][2 * c]) * (as_float(dp[2 * c]) - delta),
-                            as_float(s[i][2 * c + 1]) * (as_float(dp[2 * c + 1]) - delta));
+          ds[c] = pack_bf16_pair(mul2(pair(as_float(s[i][2 * c]), as_float(s[i][2 * c + 1])),
+                                      add2(pair(as_float(dp[2 * c]), as_float(dp[2 * c + 1])), minus_delta)));
         ptx::tmem_st_32x32b_x16(dp_tmem(slot) + lanes + columns + i * 16, ds);
       }
       ptx::tmem_wait_st();
@@ -310,7 +319,7 @@ struct KeyGradLayout {
   static constexpr int kStages = kDim == 128 ? 2 : 4;  // of Q and of dO
   static constexpr uint32_t kTileBytes = TileShape<kDim>::kBytes;
   static constexpr uint32_t kK = 0, kV = kTileBytes, kQ = 2 * kTileBytes, kDo = kQ + kStages * kTileBytes;
-  static constexpr uint32_t kStats = kDo + kStages * kTileBytes;  // [2][lse, D][128]
+  static constexpr uint32_t kStats = kDo + kStages * kTileBytes;  // [2][-lse, -D][128]
   static constexpr uint32_t kBarriers = kStats + 2 * 2 * kTile * 4;
   // kv_full, s_full, dp_full, p_ready, ds_ready, grads_full, drain, stat_full[2], stat_empty[2],
   // then q_full, q_empty, do_full, do_empty
@@ -348,19 +357,24 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const uint32_t base = ptx::smem_u32(smem_raw);
   const int warp = uniform(int32_t(threadIdx.x >> 5)), lane = threadIdx.x & 31;
 
-  // the first keys, which the most queries see, come first
+  // first chunks come first, last chunks, which few key tiles have, last
   const int32_t tile_tokens = kTile >> a.pack_shift;
   int32_t at = int32_t(blockIdx.x);
   const int32_t kv_head = at % a.kv_heads;
   at /= a.kv_heads;
-  const int32_t b = at % a.batch, key_tile = at / a.batch, k0 = key_tile * kTile;
+  const int32_t b = at % a.batch;
+  at /= a.batch;
+  const int32_t key_tile = at % ba.key_tiles, chunk = at / ba.key_tiles, k0 = key_tile * kTile;
   const Sequence seq = sequence(a, b);
   if (k0 >= seq.kl) return;
   const QueryTiles tiles(a, seq, key_tile, tile_tokens);
   const int32_t group = a.q_heads / a.kv_heads, packs = group >> a.pack_shift, head_base = kv_head * group;
-  const int32_t total = tiles.count * packs;
-  auto first_token = [&](int32_t j) { return (tiles.first + j % tiles.count) * tile_tokens; };
-  auto first_head = [&](int32_t j) { return head_base + ((j / tiles.count) << a.pack_shift); };
+  const int32_t all = tiles.count * packs, chunks = (all + ba.chunk - 1) / ba.chunk;
+  if (chunk > 0 && chunk >= chunks) return;
+  // this block's part: query tiles [j0, j0 + total) of the list (token tiles of one head pack after another)
+  const int32_t j0 = chunk * ba.chunk, total = min(all - j0, ba.chunk);
+  auto first_token = [&](int32_t j) { return (tiles.first + (j0 + j) % tiles.count) * tile_tokens; };
+  auto first_head = [&](int32_t j) { return head_base + (((j0 + j) / tiles.count) << a.pack_shift); };
 
   const uint32_t bars = base + Layout::kBarriers;
   const uint32_t kv_full = bars, s_full = bars + 8, dp_full = bars + 16, p_ready = bars + 24, ds_ready = bars + 32;
@@ -466,7 +480,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       unwound = !ok;
     }
   } else if (warp == 3) {
-    // lse (in log2 units) and D of the rows of every query tile, two tiles ahead at most
+    // -lse (in log2 units) and -D of the rows of every query tile, two tiles ahead at most
     bool ok = true;
     for (int32_t j = 0; j < total; ++j) {
       const int32_t t0 = first_token(j), head = first_head(j);
@@ -476,9 +490,9 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const int32_t r = i * 32 + lane, token = t0 + (r >> a.pack_shift);
         const int64_t stat = int64_t(head + (r & (a.pack - 1))) * a.q_rows + seq.q0 + token;
         const bool there = token < seq.ql;
-        lse[i] = there ? ba.lse[stat] * kLog2e : INFINITY;
-        delta[i] = there ? ba.delta[stat] : 0.0f;
-        if (lse[i] == -INFINITY) lse[i] = INFINITY;  // a row that sees nothing: every weight is exp(-inf)
+        lse[i] = there ? -ba.lse[stat] * kLog2e : -INFINITY;
+        delta[i] = there ? -ba.delta[stat] : 0.0f;
+        if (lse[i] == INFINITY) lse[i] = -INFINITY;  // a row that sees nothing: every weight is exp(-inf)
       }
       if (!(ok = warp_wait(stat_empty(j & 1), ((j >> 1) & 1) ^ 1u, a.wait, kSiteSmemEmpty))) break;
       float* mine = stats + (j & 1) * 2 * kTile;
@@ -498,6 +512,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     // the tokens that see this key: [from, to)
     const int32_t from = a.causal ? key - seq.off : 0;
     const int32_t to = key >= seq.kl ? 0 : a.causal && a.window > 0 && key >= a.sinks ? min(seq.ql, key + a.window - seq.off) : seq.ql;
+    const uint64_t scale2 = pair(a.scale_log2, a.scale_log2);
     bool ok = true;
     for (int32_t j = 0; j < total; ++j) {
       const uint32_t stage = j % kStages;
@@ -517,14 +532,17 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       ptx::tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float4* lse = reinterpret_cast<const float4*>(mine + columns + i * 32);
+        const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(mine + columns + i * 32);
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const float4 v = lse[c / 4];
-          p[i][c] = __float_as_uint(exp2_approx(fmaf(as_float(p[i][c]), a.scale_log2, -v.x)));
-          p[i][c + 1] = __float_as_uint(exp2_approx(fmaf(as_float(p[i][c + 1]), a.scale_log2, -v.y)));
-          p[i][c + 2] = __float_as_uint(exp2_approx(fmaf(as_float(p[i][c + 2]), a.scale_log2, -v.z)));
-          p[i][c + 3] = __float_as_uint(exp2_approx(fmaf(as_float(p[i][c + 3]), a.scale_log2, -v.w)));
+          const ulonglong2 v = lse[c / 4];
+          float x, y;
+          unpair(fma2(pair(as_float(p[i][c]), as_float(p[i][c + 1])), scale2, v.x), x, y);
+          p[i][c] = __float_as_uint(exp2_approx(x));
+          p[i][c + 1] = __float_as_uint(exp2_approx(y));
+          unpair(fma2(pair(as_float(p[i][c + 2]), as_float(p[i][c + 3])), scale2, v.y), x, y);
+          p[i][c + 2] = __float_as_uint(exp2_approx(x));
+          p[i][c + 3] = __float_as_uint(exp2_approx(y));
         }
       }
       if (masked) {
@@ -561,22 +579,24 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         uint32_t dp[32], ds[16];
         ptx::tmem_ld_32x32b_x32(dp_tmem + lanes + columns + i * 32, dp);
         ptx::tmem_wait_ld();
-        const float4* delta = reinterpret_cast<const float4*>(mine + kTile + columns + i * 32);
+        const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(mine + kTile + columns + i * 32);
+        uint64_t d[16];
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 v = delta[c / 4];
-          dp[c] = __float_as_uint(as_float(dp[c]) - v.x);
-          dp[c + 1] = __float_as_uint(as_float(dp[c + 1]) - v.y);
-          dp[c + 2] = __float_as_uint(as_float(dp[c + 2]) - v.z);
-          dp[c + 3] = __float_as_uint(as_float(dp[c + 3]) - v.w);
+        for (int c = 0; c < 16; c += 2) {
+          const ulonglong2 v = delta[c / 2];
+          d[c] = add2(pair(as_float(dp[2 * c]), as_float(dp[2 * c + 1])), v.x);
+          d[c + 1] = add2(pair(as_float(dp[2 * c + 2]), as_float(dp[2 * c + 3])), v.y);
         }
-        if (masked) {
+        if (masked) {  // dP of a pair that does not count can be anything
 #pragma unroll
-          for (int c = 0; c < 32; ++c) dp[c] = p[i][c] != 0u ? dp[c] : 0u;
+          for (int c = 0; c < 16; ++c) {
+            float x, y;
+            unpair(d[c], x, y);
+            d[c] = pair(p[i][2 * c] != 0u ? x : 0.0f, p[i][2 * c + 1] != 0u ? y : 0.0f);
+          }
         }
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          ds[c] = pack_bf16(as_float(p[i][2 * c]) * as_float(dp[2 * c]), as_float(p[i][2 * c + 1]) * as_float(dp[2 * c + 1]));
+        for (int c = 0; c < 16; ++c) ds[c] = pack_bf16_pair(mul2(pair(as_float(p[i][2 * c]), as_float(p[i][2 * c + 1])), d[c]));
         ptx::tmem_st_32x32b_x16(dp_tmem + lanes + columns + i * 16, ds);
       }
       ptx::tmem_wait_st();
@@ -605,9 +625,16 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = 0u;
             }
-            if (mine)
+            if (!mine) continue;
+            if (chunks > 1) {
+              const int64_t slot = ((int64_t(b) * a.kv_heads + kv_head) * ba.key_tiles + key_tile) * ba.max_chunks + chunk;
+              uint4* to4 = reinterpret_cast<uint4*>(ba.partial + ((slot * 2 + which) * kTile + row) * kDim + column);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) to4[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            } else {
               store_row32((which ? ba.dk + kv_row * ba.dk_stride : ba.dv + kv_row * ba.dv_stride) + int64_t(kv_head) * kDim + column,
                           v, which ? a.scale : 1.0f);
+            }
           }
       }
     }
@@ -622,6 +649,40 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   if (warp == 2) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Sums the chunks of a key tile in their order.  A block per key tile, four columns per thread and step.
+template <int kDim>
+__global__ void __launch_bounds__(256) attention_key_grad_join_kernel(const __grid_constant__ BackwardArgs ba) {
+  const Args& a = ba.f;
+  int32_t at = int32_t(blockIdx.x);
+  const int32_t kv_head = at % a.kv_heads;
+  at /= a.kv_heads;
+  const int32_t b = at % a.batch, key_tile = at / a.batch, k0 = key_tile * kTile;
+  const Sequence seq = sequence(a, b);
+  if (k0 >= seq.kl) return;
+  const int32_t all = QueryTiles(a, seq, key_tile, kTile >> a.pack_shift).count * ((a.q_heads / a.kv_heads) >> a.pack_shift);
+  const int32_t chunks = (all + ba.chunk - 1) / ba.chunk;
+  if (chunks <= 1) return;
+  const int64_t slot = ((int64_t(b) * a.kv_heads + kv_head) * ba.key_tiles + key_tile) * ba.max_chunks;
+  const int32_t rows = min(kTile, seq.kl - k0);
+  constexpr int kVectors = kDim / 4;
+  for (int32_t i = int32_t(blockIdx.y) * 256 + threadIdx.x; i < 2 * rows * kVectors; i += int32_t(gridDim.y) * 256) {
+    const int32_t which = i / (rows * kVectors), rest = i - which * rows * kVectors, row = rest / kVectors, column = rest % kVectors * 4;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float* from = ba.partial + ((slot * 2 + which) * kTile + row) * kDim + column;
+    for (int32_t c = 0; c < chunks; ++c) {
+      const float4 v = *reinterpret_cast<const float4*>(from + int64_t(c) * 2 * kTile * kDim);
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+    const float scale = which ? a.scale : 1.0f;
+    const int64_t kv_row = int64_t(seq.k0) + k0 + row;
+    uint16_t* to = (which ? ba.dk + kv_row * ba.dk_stride : ba.dv + kv_row * ba.dv_stride) + int64_t(kv_head) * kDim + column;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(sum.x * scale, sum.y * scale), pack_bf16(sum.z * scale, sum.w * scale));
   }
 }
 

@@ -203,7 +203,5 @@ def test_attention_without_work_or_support():
     assert api.launch_attention(attention_params(batch=0, q=None)) == 0
     assert api.launch_attention(attention_params(q_len=0, q=None)) == 0
     assert api.launch_attention_backward(attention_backward_params(batch=0)) == 0
-    rc, size = api.attention_backward_workspace_size(attention_backward_params())
-    assert rc == 0 and size >= 8 * 256 * 4
     assert N.lib().fuse_b200_launch_attention(None, None, None) == INVALID
     assert N.lib().fuse_b200_launch_attention_backward(None, None, None) == INVALID
