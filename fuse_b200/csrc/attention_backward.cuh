@@ -9,8 +9,10 @@
 // are computed in both: seven products instead of the five of a single pass, but every sum stays in TMEM in a fixed
 // order -- no atomics, the same bits every time, no FP32 copy of dQ in memory.
 //
-// Roles as in the forward kernel: loads, UMMA issue, TMEM, and eight warps of elementwise work, four per half of
-// the columns, one thread per row and half.  P and dS are rounded to BF16 for their products, as every operand of
+// Roles as in the forward kernel: loads, UMMA issue, TMEM, and eight warps of elementwise work, four per half of the
+// columns, one thread per row and half.  The first kernel's dQ has an issuing warp of its own (192 -> 187 us at
+// 8192 x 8 heads); the second kernel's four products keep one order, dV, S of the next tile, dK, dP of the next (two
+// warps: 245 -> 319 us).  P and dS are rounded to BF16 for their products, as every operand of
 // the tensor cores is; they are made from FP32 scores and dP and accumulated in FP32.
 #pragma once
 
@@ -57,8 +59,8 @@ struct QueryGradLayout {
   static constexpr uint32_t kTileBytes = TileShape<kDim>::kBytes;
   static constexpr uint32_t kQ = 0, kDo = kTileBytes, kK = 2 * kTileBytes, kV = kK + kKStages * kTileBytes;
   static constexpr uint32_t kBarriers = kV + kVStages * kTileBytes;
-  // q_full, s_full, s_read, dp_full[2], ds_ready[2], dq_full, drain, then k_full, k_empty, v_full, v_empty
-  static constexpr uint32_t kNumBarriers = 9 + 2 * kKStages + 2 * kVStages;
+  // q_full, s_full, s_read, dp_full[2], ds_ready[2], ds_read[2], dq_full, drain[2], then k_full, k_empty, v_full, v_empty
+  static constexpr uint32_t kNumBarriers = 12 + 2 * kKStages + 2 * kVStages;
   static constexpr uint32_t kSlot = kBarriers + kNumBarriers * 8;
   static constexpr uint32_t kDelta = (kSlot + 16 + 15) / 16 * 16;  // [2][128] partial sums
   static constexpr uint32_t kDynamicBytes = kDelta + 1024 + 1024;
@@ -92,13 +94,15 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   const TileList tiles(KeyRange(a, seq, first, last));
 
   const uint32_t bars = base + Layout::kBarriers;
-  const uint32_t q_full = bars, s_full = bars + 8, s_read = bars + 16, dq_full = bars + 56, drain = bars + 64;
-  auto dp_full = [&](uint32_t i) { return bars + 24u + 8u * i; };
-  auto ds_ready = [&](uint32_t i) { return bars + 40u + 8u * i; };
-  auto k_full = [&](uint32_t s) { return bars + 8u * (9 + s); };
-  auto k_empty = [&](uint32_t s) { return bars + 8u * (9 + kKStages + s); };
-  auto v_full = [&](uint32_t s) { return bars + 8u * (9 + 2 * kKStages + s); };
-  auto v_empty = [&](uint32_t s) { return bars + 8u * (9 + 2 * kKStages + kVStages + s); };
+  const uint32_t q_full = bars, s_full = bars + 8, s_read = bars + 16, dq_full = bars + 72;
+  auto dp_full = [&](uint32_t i) { return bars + 8u * (3 + i); };
+  auto ds_ready = [&](uint32_t i) { return bars + 8u * (5 + i); };
+  auto ds_read = [&](uint32_t i) { return bars + 8u * (7 + i); };
+  auto drain = [&](uint32_t i) { return bars + 8u * (10 + i); };
+  auto k_full = [&](uint32_t s) { return bars + 8u * (12 + s); };
+  auto k_empty = [&](uint32_t s) { return bars + 8u * (12 + kKStages + s); };
+  auto v_full = [&](uint32_t s) { return bars + 8u * (12 + 2 * kKStages + s); };
+  auto v_empty = [&](uint32_t s) { return bars + 8u * (12 + 2 * kKStages + kVStages + s); };
   auto k_tile = [&](uint32_t s) { return base + Layout::kK + s * Layout::kTileBytes; };
   auto v_tile = [&](uint32_t s) { return base + Layout::kV + s * Layout::kTileBytes; };
 
@@ -113,9 +117,10 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(dp_full(i), 1);
       ptx::mbar_init(ds_ready(i), 8);
+      ptx::mbar_init(ds_read(i), 1);
+      ptx::mbar_init(drain(i), 1);
     }
     ptx::mbar_init(dq_full, 1);
-    ptx::mbar_init(drain, 1);
     for (int s = 0; s < kKStages; ++s) {
       ptx::mbar_init(k_full(s), 1);
       ptx::mbar_init(k_empty(s), 1);
@@ -157,36 +162,48 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       unwound = !ok;
     }
   } else if (warp == 1) {
+    // S and dP; the products that wait for the elementwise warps are another warp's, so neither holds the other up
     if (tiles.count > 0) {
       const uint32_t issue = ptx::elect_one();
       bool ok = warp_wait(q_full, 0, a.wait, kSiteSmemFull);
-      uint32_t ks = 0, k_phase = 0, vs = 0, v_phase = 0, last_ks = 0;
-      for (int32_t it = -1; ok && it < tiles.count; ++it) {
-        if (it + 1 < tiles.count) {  // S and dP of the next key tile
-          // S is read into registers, then its columns take the next tile's; dP alternates between two slots,
-          // whose dS the product two tiles ago has read
-          if (it >= 0 && !(ok = warp_wait(s_read, it & 1, a.wait, kSiteTmemEmpty))) break;
-          if (!(ok = warp_wait(k_full(ks), k_phase, a.wait, kSiteSmemFull))) break;
-          ptx::tc_fence_after();
-          mma_rows<kDim>(issue, s_tmem, base + Layout::kQ, k_tile(ks));
-          ptx::umma_commit_if(issue, s_full);
-          if (!(ok = warp_wait(v_full(vs), v_phase, a.wait, kSiteSmemFull))) break;
-          mma_rows<kDim>(issue, dp_tmem((it + 1) & 1), base + Layout::kDo, v_tile(vs));
-          ptx::umma_commit_if(issue, dp_full((it + 1) & 1));
-          ptx::umma_commit_if(issue, v_empty(vs));
-          if (++vs == kVStages) { vs = 0; v_phase ^= 1u; }
-        }
-        if (it >= 0) {
-          if (!(ok = warp_wait(ds_ready(it & 1), (it >> 1) & 1, a.wait, kSiteTmemEmpty))) break;
-          ptx::tc_fence_after();
-          mma_weights<kDim>(issue, dq_tmem, Halves{dp_tmem(it & 1)}, k_tile(last_ks), it > 0);
-          ptx::umma_commit_if(issue, k_empty(last_ks));
-        }
-        last_ks = ks;
+      uint32_t ks = 0, k_phase = 0, vs = 0, v_phase = 0;
+      for (int32_t it = 0; ok && it < tiles.count; ++it) {
+        if (!(ok = warp_wait(k_full(ks), k_phase, a.wait, kSiteSmemFull))) break;
+        // the last tile's S is in registers
+        if (it > 0 && !(ok = warp_wait(s_read, (it - 1) & 1, a.wait, kSiteTmemEmpty))) break;
+        ptx::tc_fence_after();
+        mma_rows<kDim>(issue, s_tmem, base + Layout::kQ, k_tile(ks));
+        ptx::umma_commit_if(issue, s_full);
         if (++ks == kKStages) { ks = 0; k_phase ^= 1u; }
+        if (!(ok = warp_wait(v_full(vs), v_phase, a.wait, kSiteSmemFull))) break;
+        // dP alternates between two slots, whose dS the product two tiles ago has read
+        if (it > 1 && !(ok = warp_wait(ds_read(it & 1), ((it >> 1) - 1) & 1, a.wait, kSiteTmemEmpty))) break;
+        mma_rows<kDim>(issue, dp_tmem(it & 1), base + Layout::kDo, v_tile(vs));
+        ptx::umma_commit_if(issue, dp_full(it & 1));
+        ptx::umma_commit_if(issue, v_empty(vs));
+        if (++vs == kVStages) { vs = 0; v_phase ^= 1u; }
       }
-      ptx::umma_commit_if(issue, ok ? dq_full : drain);
-      if (!ok) mbar_wait<false>(drain, 0u, a.wait, kSiteDrain, false);
+      if (!ok) {  // UMMAs already issued retire before TMEM is released
+        ptx::umma_commit_if(issue, drain(0));
+        mbar_wait<false>(drain(0), 0u, a.wait, kSiteDrain, false);
+      }
+      unwound = !ok;
+    }
+  } else if (warp == 2) {
+    if (tiles.count > 0) {  // dQ
+      const uint32_t issue = ptx::elect_one();
+      bool ok = true;
+      uint32_t ks = 0;
+      for (int32_t it = 0; it < tiles.count; ++it) {
+        if (!(ok = warp_wait(ds_ready(it & 1), (it >> 1) & 1, a.wait, kSiteTmemEmpty))) break;
+        ptx::tc_fence_after();
+        mma_weights<kDim>(issue, dq_tmem, Halves{dp_tmem(it & 1)}, k_tile(ks), it > 0);
+        ptx::umma_commit_if(issue, ds_read(it & 1));
+        ptx::umma_commit_if(issue, k_empty(ks));
+        if (++ks == kKStages) ks = 0;
+      }
+      ptx::umma_commit_if(issue, ok ? dq_full : drain(1));
+      if (!ok) mbar_wait<false>(drain(1), 0u, a.wait, kSiteDrain, false);
       unwound = !ok;
     }
   } else if (warp >= 4) {
