@@ -46,8 +46,15 @@ def _grad(g: torch.Tensor) -> torch.Tensor:
     return g.clone(memory_format=torch.contiguous_format)
 
 
+try:  # the stream's handle without the Stream object around it: 0.1 us instead of 1.4
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 class _On:
-    """Makes a tensor's device the current one for a launch, where it is not already."""
+    """Makes a tensor's device the current one for a launch, where it is not already, and hands out its stream."""
     __slots__ = ("index", "back")
 
     def __init__(self, t: torch.Tensor):
@@ -57,7 +64,7 @@ class _On:
         self.back = torch.cuda.current_device()
         if self.back != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.back != self.index:
@@ -323,8 +330,9 @@ def _attention_forward(q, k, v, shape, out, want_lse):
     p.output, p.output_stride = out.data_ptr(), _stride(out)
     lse = None
     if want_lse:
-        lse = torch.full((shape[3], q.shape[0]), -torch.inf, dtype=torch.float32, device=q.device) if ragged else \
-            torch.empty((shape[3], q.shape[0]), dtype=torch.float32, device=q.device)
+        lse = torch.empty((shape[3], q.shape[0]), dtype=torch.float32, device=q.device)
+        if ragged and want_lse == "whole":
+            lse.fill_(-torch.inf)
         p.lse = lse.data_ptr()
     with _On(q) as stream:
         size = C.c_size_t()
@@ -337,8 +345,12 @@ def _attention_forward(q, k, v, shape, out, want_lse):
 
 
 def _attention_backward(do, q, k, v, out, lse, shape):
+    # one allocation (and, where rows may belong to no sequence, one clearing) for the three
     make = torch.zeros if _partial(q, k, shape) or not q.shape[0] else torch.empty
-    dq, dk, dv = (make(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
+    nq, nk = q.shape[0] * q.shape[1], k.shape[0] * k.shape[1]
+    gap = -nq % 8  # the parts start on 16-byte boundaries
+    whole = make(nq + gap + 2 * nk, dtype=BF16, device=q.device)
+    dq, dk, dv = whole[:nq].view(q.shape), whole[nq + gap:nq + gap + nk].view(k.shape), whole[nq + gap + nk:].view(v.shape)
     if not q.shape[0]:
         return dq, dk, dv
     do = _grad(do)
@@ -360,8 +372,8 @@ def _attention_backward(do, q, k, v, out, lse, shape):
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, shape):
-        out, lse = _attention_forward(q, k, v, shape, None, True)
+    def forward(ctx, q, k, v, shape, want_lse):
+        out, lse = _attention_forward(q, k, v, shape, None, want_lse)
         ctx.save_for_backward(q, k, v, out, lse, *shape[10:])
         ctx.shape = shape[:10]
         ctx.mark_non_differentiable(lse)
@@ -372,7 +384,7 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, do, _lse):
         q, k, v, out, lse, *rows = ctx.saved_tensors
         dq, dk, dv = _attention_backward(do, q, k, v, out, lse, (*ctx.shape, *rows))
-        return dq, dk, dv, None
+        return dq, dk, dv, None, None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: int, batch: int = 1, causal: bool = True,
@@ -409,7 +421,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
     if _wants_grad(q, k, v):
         if out is not None:
             raise RuntimeError("out= would be overwritten before the backward has read it: leave it out, or use torch.no_grad()")
-        out, lse = _Attention.apply(q, k, v, shape)
+        out, lse = _Attention.apply(q, k, v, shape, "whole" if return_lse else "own")
     else:
-        out, lse = _attention_forward(q, k, v, shape, out, return_lse)
+        out, lse = _attention_forward(q, k, v, shape, out, "whole" if return_lse else None)
     return (out, lse) if return_lse else out

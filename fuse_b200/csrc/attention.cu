@@ -48,7 +48,7 @@ int32_t plan_splits(const fuse_b200_attention_params& p, int sm_count) {
   if (p.window > 0 && seen < keys) keys = seen + (p.sinks < keys - seen ? p.sinks : keys - seen);
   const int64_t tiles = (keys + attn::kTile - 1) / attn::kTile + (p.window > 0 ? 1 : 0);
   if (blocks == 0 || blocks >= sm_count || tiles < 4) return 1;
-  constexpr double kFixed = 3.0, kJoin = 2.0;
+  constexpr double kFixed = 5.0, kJoin = 2.0;
   double best = double(tiles) + kFixed;
   int32_t splits = 1;
   for (int64_t s = 2; s <= tiles && s <= 256; ++s) {
@@ -61,9 +61,14 @@ int32_t plan_splits(const fuse_b200_attention_params& p, int sm_count) {
   }
   return splits;
 }
+// The whole of the queries is one tile per head pack and batch item: both tiles of a block work on it.
+bool pair_tiles(const fuse_b200_attention_params& p, int32_t splits) {
+  return splits > 1 && p.q_len <= attn::kTile / packed_heads(p);
+}
 size_t cells(const fuse_b200_attention_params& p) { return size_t(p.batch) * size_t(p.q_len) * size_t(p.q_heads); }
 size_t split_bytes(const fuse_b200_attention_params& p, int32_t splits) {
-  return splits > 1 ? size_t(splits) * cells(p) * size_t(p.head_dim + 1) * sizeof(float) : 0;
+  const size_t parts = size_t(splits) * (pair_tiles(p, splits) ? 2 : 1);
+  return splits > 1 ? parts * cells(p) * size_t(p.head_dim + 1) * sizeof(float) : 0;
 }
 
 cudaError_t workspace_size(const fuse_b200_attention_params& p, size_t* bytes) {
@@ -98,7 +103,7 @@ attn::Args fill_args(const fuse_b200_attention_params& p) {
   a.scale_log2 = p.scale * attn::kLog2e;
   a.out = p.output;
   a.lse = p.lse;
-  a.splits = 1;
+  a.splits = a.parts = 1;
   return a;
 }
 
@@ -142,12 +147,14 @@ cudaError_t attention(const fuse_b200_attention_params& p, const fuse_b200_optio
   attn::Args a = fill_args(p);
   a.out_stride = out_stride;
   a.splits = plan_splits(p, info.sm_count);
+  a.paired = pair_tiles(p, a.splits) ? 1 : 0;
+  a.parts = a.paired ? 2 * a.splits : a.splits;
   if (a.splits > 1) {
     if (p.workspace == nullptr || reinterpret_cast<uintptr_t>(p.workspace) % 256 != 0 ||
         p.workspace_bytes < split_bytes(p, a.splits))
       return cudaErrorInvalidValue;
     a.partial = static_cast<float*>(p.workspace);
-    a.partial_lse = a.partial + size_t(a.splits) * cells(p) * p.head_dim;
+    a.partial_lse = a.partial + size_t(a.parts) * cells(p) * p.head_dim;
   }
   a.wait = host::make_wait(info, 0, options ? options->wait_budget_ns : 0);
   return p.head_dim == 128 ? launch_forward<128>(p, a, q_stride, k_stride, v_stride, stream)

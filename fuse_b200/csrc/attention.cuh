@@ -20,6 +20,10 @@
 // work for the other.  They execute in issue order, so S may overwrite the P that the UMMA before it reads, and "S of
 // the next keys is complete" implies "O holds all keys before", which is what a softmax group needs to rescale O in place.
 //
+// Few queries (one tile of them) against many keys: the keys are split over blocks, and within a block both tiles hold
+// the same queries and take every other key tile, so that one's softmax overlaps the other's products and the loads keep
+// coming.  Every part leaves its normalised O and its lse, and a second kernel joins them.
+//
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then
 // stay below 2^8 in BF16 and the sums below 2^8 kv_len in FP32; the result is divided by the same sum, so
 // this changes no value beyond rounding).  S, the statistics and O are FP32; P is rounded to BF16 for the
@@ -47,8 +51,10 @@ struct Args {
   uint16_t* out;
   int64_t out_stride;
   float* lse;  // [q_heads][q_rows] or nullptr
-  // split over keys: partial results per (split, batch, token, head), joined by a second kernel
-  int32_t splits;
+  // split over keys: partial results per (part, batch, token, head), joined by a second kernel
+  int32_t splits;  // blocks along the keys
+  int32_t paired;  // one query tile a block: both of its tiles work on it, on every other key tile
+  int32_t parts;   // splits, times two when paired
   float *partial, *partial_lse;
 };
 
@@ -283,14 +289,17 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int32_t pack = at % packs;
   at /= packs;
   const int32_t b = at % a.batch;
-  const int32_t token_blocks = (a.q_len + 2 * tile_tokens - 1) / (2 * tile_tokens);
-  const int32_t t0 = (token_blocks - 1 - at / a.batch) * 2 * tile_tokens;
+  const int32_t second = a.paired ? 0 : tile_tokens;  // from the first tile's tokens to the other's
+  const int32_t token_blocks = (a.q_len + tile_tokens + second - 1) / (tile_tokens + second);
+  const int32_t t0 = (token_blocks - 1 - at / a.batch) * (tile_tokens + second);
   const Sequence seq = sequence(a, b);
   if (t0 >= seq.ql) return;  // (the whole block, before anything is set up)
   const int32_t head0 = pack << a.pack_shift, kv_head = head0 / (a.q_heads / a.kv_heads);
-  const int32_t first[2] = {t0, t0 + tile_tokens};
-  const int32_t last[2] = {min(t0 + tile_tokens, seq.ql), min(t0 + 2 * tile_tokens, seq.ql)};
-  const KeyRange range(a, seq, t0, last[1]);
+  const KeyRange range(a, seq, t0, min(t0 + second + tile_tokens, seq.ql));
+  // whether tile t, which sees the keys `own`, works on the key tile of iteration `it`
+  auto works = [&](int t, const KeyRange& own, const TileList& list, int32_t it, int32_t first_it) {
+    return own.sees(list.tile(it) * kTile, kTile) && (!a.paired || ((it - first_it) & 1) == t);
+  };
   const TileList tiles(range);
   const int32_t per_split = (tiles.count + a.splits - 1) / a.splits;
   const int32_t it0 = min(split * per_split, tiles.count), it1 = min(it0 + per_split, tiles.count);
@@ -346,9 +355,9 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (lane == 0 && it0 < it1) {
       bool ok = true;
       auto load_q = [&](int t) {
-        if (first[t] >= last[t]) return;
+        if (t0 + t * second >= seq.ql) return;
         ptx::mbar_expect_tx(q_full(t), Layout::kTileBytes);
-        load_tile<kDim>(base + t * Layout::kTileBytes, &map_q, q_full(t), head0, seq.q0 + first[t]);
+        load_tile<kDim>(base + t * Layout::kTileBytes, &map_q, q_full(t), head0, seq.q0 + t0 + t * second);
       };
       load_q(0);
       for (int32_t it = it0; ok && it < it1; ++it) {
@@ -372,10 +381,10 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const int t = warp >> 1;
     if (it0 < it1) {
       const uint32_t issue = ptx::elect_one();
-      const int32_t my_first = t0 + t * tile_tokens;
+      const int32_t my_first = t0 + t * second;
       const KeyRange own(a, seq, my_first, min(my_first + tile_tokens, seq.ql));
       const uint32_t q_tile = base + t * Layout::kTileBytes;
-      auto seen = [&](int32_t it) { return it < it1 && own.sees(tiles.tile(it) * kTile, kTile); };
+      auto seen = [&](int32_t it) { return it < it1 && works(t, own, tiles, it, it0); };
       bool ok = my_first >= seq.ql || warp_wait(q_full(t), 0, a.wait, kSiteSmemFull);
       uint32_t p_phase = 0, has_o = 0;
       uint32_t s = 0, s_next = 0, v_phase = 0, k_phase = 0;  // stages of V of tile `it` and of K of tile it + 1
@@ -410,7 +419,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     ptx::setmaxnreg_inc<208>();
     const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const int32_t my_first = t ? t0 + tile_tokens : t0, my_last = min(my_first + tile_tokens, seq.ql);
+    const int32_t my_first = t ? t0 + second : t0, my_last = min(my_first + tile_tokens, seq.ql);
     const KeyRange my_range(a, seq, my_first, my_last);
     const uint32_t o_at = o_tmem(t) + lanes;
     const int32_t token = my_first + (row >> a.pack_shift), head = head0 + (row & (a.pack - 1));
@@ -425,7 +434,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint32_t phase = 0;
     for (int32_t it = it0; ok && it < it1; ++it) {
       const int32_t k0 = tiles.tile(it) * kTile;
-      if (!my_range.sees(k0, kTile)) continue;
+      if (!works(t, my_range, tiles, it, it0)) continue;
       if (!(ok = warp_wait(s_full(t), phase, a.wait, kSiteTmemFull))) break;
       phase ^= 1u;
       ptx::tc_fence_after();
@@ -511,9 +520,10 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const float lse = seen ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
       const int64_t out_row = int64_t(seq.q0) + token;
       if (ok) {
-        const int64_t cell = ((int64_t(split) * a.batch + b) * a.q_len + token) * a.q_heads + head;
+        const int32_t part = a.paired ? 2 * split + t : split;
+        const int64_t cell = ((int64_t(part) * a.batch + b) * a.q_len + token) * a.q_heads + head;
         if (mine) {
-          if (a.splits > 1) a.partial_lse[cell] = lse;
+          if (a.parts > 1) a.partial_lse[cell] = lse;
           else if (a.lse != nullptr) a.lse[int64_t(head) * a.q_rows + out_row] = lse;
         }
 #pragma unroll
@@ -524,7 +534,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = seen ? __float_as_uint(as_float(o[i]) * inverse) : 0u;
           if (!mine) continue;
-          if (a.splits > 1) {
+          if (a.parts > 1) {
             uint4* to = reinterpret_cast<uint4*>(a.partial + cell * kDim + c);
 #pragma unroll
             for (int i = 0; i < 8; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -554,7 +564,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   }
 }
 
-// Joins the splits: one warp per (token, head).
+// Joins the parts: one warp per (token, head).
 //   m = max lse_s, w_s = exp(lse_s - m), O = sum w_s O_s / sum w_s, lse = m + log sum w_s
 template <int kDim>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ Args a) {
@@ -567,14 +577,14 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   const Sequence seq = sequence(a, int32_t(cell / a.q_heads / a.q_len));
   if (token >= seq.ql) return;
   float m = -INFINITY;
-  for (int32_t s = lane; s < a.splits; s += 32) m = fmaxf(m, a.partial_lse[s * cells + cell]);
+  for (int32_t s = lane; s < a.parts; s += 32) m = fmaxf(m, a.partial_lse[s * cells + cell]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float sum = 0.0f, acc[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) acc[i] = 0.0f;
   const float ref = m == -INFINITY ? 0.0f : m;
-  for (int32_t s = 0; s < a.splits; ++s) {
+  for (int32_t s = 0; s < a.parts; ++s) {
     const float w = exp2_approx((a.partial_lse[s * cells + cell] - ref) * kLog2e);
     if (w == 0.0f) continue;  // (the same for the whole warp)
     sum += w;

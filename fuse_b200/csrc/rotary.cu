@@ -7,10 +7,9 @@
 // The angle of a far position needs more than FP32: p f_i may be 10^5 turns, of which only the
 // fraction matters.  Positions are whole numbers, so the fraction of p f_i / 2 pi is p times the
 // 64-bit fraction of f_i / 2 pi modulo 2^64: one integer product, exact but for the rounding of the
-// frequency itself (p 2^-65 turns).  Its high word, as a signed fraction of a half turn, goes to
-// sincospif.
+// frequency itself (p 2^-65 turns).  Its high word is the angle as a signed fraction of a half turn.
 //
-// Bound by HBM: 2 bytes read and 2 written per element.  A block takes kTokens rows at a time, computes
+// Bound by HBM: 2 bytes read and 2 written per element.  A block takes a few rows at a time, computes
 // their cosines and sines once into shared memory (they serve every head) and then walks the rows'
 // heads in items of sixteen elements, two 16-byte loads and stores each.
 #include "launch.cuh"
@@ -37,15 +36,16 @@ struct RotaryArgs {
 
 // `within`: the row's place in its sequence, counted on from a row that lies in it (one division for
 // all rows of a block; only rows behind the sequence's end divide again).
-__device__ __forceinline__ float2 pair_rotation(const RotaryArgs& a, int64_t row, int64_t within, int32_t pair) {
+__device__ __forceinline__ float2 pair_rotation(const RotaryArgs& a, int64_t row, int64_t within, uint64_t per_position) {
   int64_t p;
   if (a.positions == nullptr) p = a.start + (within < a.seq_len ? within : within % a.seq_len);
   else if (a.position_bytes == 4) p = static_cast<const int32_t*>(a.positions)[row];
   else p = static_cast<const int64_t*>(a.positions)[row];
-  const uint64_t turn = uint64_t(p) * a.turns[pair];
-  float s, c;
-  sincospif(float(int32_t(turn >> 32)) * 4.656612873077392578125e-10f /* 2^-31 */, &s, &c);
-  return make_float2(c * a.magnitude, s * a.sine);
+  const uint64_t turn = uint64_t(p) * per_position;
+  // |angle| <= pi, where the hardware's sine and cosine are within 2^-21.1 (absolute): far below the
+  // BF16 step of what they multiply (2^-9 of it)
+  const float angle = float(int32_t(turn >> 32)) * 1.46291807926715968e-9f /* pi 2^-31 */;
+  return make_float2(__cosf(angle) * a.magnitude, __sinf(angle) * a.sine);
 }
 
 __device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
@@ -58,61 +58,88 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 
 // An item is 16 elements of one head: with the half layout eight of the first half and the eight they
 // pair with, with the interleaved layout (and in the part that is only copied) sixteen neighbours.
+// A thread keeps one item of the row and goes from row to row, kBatch rows' loads in flight at a time.
+constexpr int kBlock = 256, kBatch = 2, kResident = 4;
 template <bool kInterleaved>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryArgs a, int32_t tokens) {
-  extern __shared__ float2 turn[];  // [tokens][pairs]
+__global__ void __launch_bounds__(kBlock, kResident) rotary_kernel(const __grid_constant__ RotaryArgs a, int32_t tokens) {
+  // [tokens][4][rotated items]: cosine and sine of pairs 2j and 2j + 1 of an item, neighbouring items side by side
+  extern __shared__ float4 turn[];
+  // lanes that index the kernel's parameters apart from one another are served one by one (97 us against 77 for 128K rows of five heads of 128)
+  __shared__ uint64_t per_position[kMaxPairs];
+  if (threadIdx.x < kMaxPairs) per_position[threadIdx.x] = a.turns[threadIdx.x];
+  __syncthreads();
   const int32_t pairs = a.rotary_dim >> 1, heads = a.q_heads + a.kv_heads;
   const int32_t rotated = a.rotary_dim >> 4;                  // items of a head that turn
-  const int32_t items = a.head_dim >> 4;
+  const int32_t items = a.head_dim >> 4, slots = heads * items;
+  const int32_t rows_at_once = slots < kBlock ? kBlock / slots : 1;
+  const int32_t first_row = slots < kBlock ? int32_t(threadIdx.x) / slots : 0;
+  const int32_t first_slot = int32_t(threadIdx.x) - first_row * (slots < kBlock ? slots : 0);
+  // a thread's pair, and the first and further rows whose angles it computes
+  const int32_t turns_at_once = kBlock / pairs, first_turn = int32_t(threadIdx.x) / pairs, pair = int32_t(threadIdx.x) - first_turn * pairs;
+  const int32_t turn_at = ((pair & 7) >> 1) * (2 * rotated) + (pair >> 3) * 2 + (pair & 1);
+  const uint64_t mine = per_position[pair];
   const int64_t chunks = (a.rows + tokens - 1) / tokens;
   for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int64_t row0 = chunk * tokens;
     const int32_t n = int32_t(a.rows - row0 < tokens ? a.rows - row0 : tokens);
-    const int64_t within0 = row0 % a.seq_len;
-    for (int32_t i = threadIdx.x; i < n * pairs; i += blockDim.x) {
-      const int32_t token = i / pairs;
-      turn[i] = pair_rotation(a, row0 + token, within0 + token, i - token * pairs);
-    }
+    const int64_t within0 = a.positions == nullptr ? row0 % a.seq_len : 0;
+    for (int32_t token = first_turn; token < n; token += turns_at_once)
+      if (first_turn < turns_at_once)
+        reinterpret_cast<float2*>(turn)[token * pairs + turn_at] = pair_rotation(a, row0 + token, within0 + token, mine);
     __syncthreads();
-    for (int32_t i = threadIdx.x; i < n * heads * items; i += blockDim.x) {
-      const int32_t item = i % items, at = i / items, head = at % heads, token = at / heads;
-      const int64_t row = row0 + token;
-      const bool is_q = head < a.q_heads;
-      const uint16_t* in = is_q ? a.q + row * a.q_stride + int64_t(head) * a.head_dim
-                                : a.k + row * a.k_stride + int64_t(head - a.q_heads) * a.head_dim;
-      uint16_t* out = is_q ? a.qo + row * a.qo_stride + int64_t(head) * a.head_dim
-                           : a.ko + row * a.ko_stride + int64_t(head - a.q_heads) * a.head_dim;
-      int32_t first, second;
-      if (kInterleaved || item >= rotated) {
-        first = item * 16;
-        second = first + 8;
-      } else {
-        first = item * 8;
-        second = first + pairs;
-      }
-      uint4 u = *reinterpret_cast<const uint4*>(in + first), v = *reinterpret_cast<const uint4*>(in + second);
-      if (item < rotated) {
-        uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
-        uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
-        const float4* cs = reinterpret_cast<const float4*>(turn + token * pairs + item * 8);
+    for (int32_t slot = first_row < rows_at_once ? first_slot : slots; slot < slots; slot += kBlock) {
+      const int32_t head = slot / items, item = slot - head * items;
+      const bool is_q = head < a.q_heads, turned = item < rotated;
+      const int64_t in_stride = is_q ? a.q_stride : a.k_stride, out_stride = is_q ? a.qo_stride : a.ko_stride;
+      const int64_t column = int64_t(is_q ? head : head - a.q_heads) * a.head_dim;
+      const int32_t first = kInterleaved || !turned ? item * 16 : item * 8;
+      const int32_t second = kInterleaved || !turned ? first + 8 : first + pairs;
+      const uint16_t* in = (is_q ? a.q : a.k) + (row0 + first_row) * in_stride + column + first;
+      uint16_t* out = (is_q ? a.qo : a.ko) + (row0 + first_row) * out_stride + column + first;
+      const int64_t in_step = rows_at_once * in_stride, out_step = rows_at_once * out_stride;
+      const int32_t apart = second - first;
+      for (int32_t token0 = first_row; token0 < n; token0 += kBatch * rows_at_once) {
+        uint4 us[kBatch], vs[kBatch];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 t = cs[j];  // cosine and sine of pairs 2j and 2j + 1 of this item
-          if constexpr (kInterleaved) {
-            uint32_t& w0 = j < 2 ? uw[2 * j] : vw[2 * j - 4];
-            uint32_t& w1 = j < 2 ? uw[2 * j + 1] : vw[2 * j - 3];
-            const float a0 = low(w0), b0 = high(w0), a1 = low(w1), b1 = high(w1);
-            w0 = pack(a0 * t.x - b0 * t.y, a0 * t.y + b0 * t.x);
-            w1 = pack(a1 * t.z - b1 * t.w, a1 * t.w + b1 * t.z);
-          } else {
-            const float a0 = low(uw[j]), a1 = high(uw[j]), b0 = low(vw[j]), b1 = high(vw[j]);
-            uw[j] = pack(a0 * t.x - b0 * t.y, a1 * t.z - b1 * t.w);
-            vw[j] = pack(a0 * t.y + b0 * t.x, a1 * t.w + b1 * t.z);
+        for (int k = 0; k < kBatch; ++k) {
+          const int32_t token = token0 + k * rows_at_once;
+          if (token < n) {
+            us[k] = *reinterpret_cast<const uint4*>(in);
+            vs[k] = *reinterpret_cast<const uint4*>(in + apart);
           }
+          in += in_step;
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int32_t token = token0 + k * rows_at_once;
+          if (token >= n) break;
+          uint4 &u = us[k], &v = vs[k];
+          if (turned) {
+            uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+            const float4* cs = turn + token * (pairs >> 1) + item;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 t = cs[j * rotated];  // cosine and sine of pairs 2j and 2j + 1 of this item
+              if constexpr (kInterleaved) {
+                uint32_t& w0 = j < 2 ? uw[2 * j] : vw[2 * j - 4];
+                uint32_t& w1 = j < 2 ? uw[2 * j + 1] : vw[2 * j - 3];
+                const float a0 = low(w0), b0 = high(w0), a1 = low(w1), b1 = high(w1);
+                w0 = pack(a0 * t.x - b0 * t.y, a0 * t.y + b0 * t.x);
+                w1 = pack(a1 * t.z - b1 * t.w, a1 * t.w + b1 * t.z);
+              } else {
+                const float a0 = low(uw[j]), a1 = high(uw[j]), b0 = low(vw[j]), b1 = high(vw[j]);
+                uw[j] = pack(a0 * t.x - b0 * t.y, a1 * t.z - b1 * t.w);
+                vw[j] = pack(a0 * t.y + b0 * t.x, a1 * t.w + b1 * t.z);
+              }
+            }
+            u = make_uint4(uw[0], uw[1], uw[2], uw[3]);
+            v = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+          }
+          *reinterpret_cast<uint4*>(out) = u;
+          *reinterpret_cast<uint4*>(out + apart) = v;
+          out += out_step;
         }
       }
-      *reinterpret_cast<uint4*>(out + first) = u;
-      *reinterpret_cast<uint4*>(out + second) = v;
     }
     __syncthreads();
   }
@@ -127,7 +154,7 @@ __global__ void __launch_bounds__(256) rotary_pairs_kernel(const __grid_constant
     const int64_t row = i / slots;
     const int32_t slot = int32_t(i - row * slots);
     const bool turned = slot < pairs;
-    const float2 t = turned ? pair_rotation(a, row, row, slot) : make_float2(1.0f, 0.0f);
+    const float2 t = turned ? pair_rotation(a, row, row, a.turns[slot]) : make_float2(1.0f, 0.0f);
     const int32_t first = !turned ? a.rotary_dim + slot - pairs : interleaved ? 2 * slot : slot;
     const int32_t second = interleaved ? first + 1 : first + pairs;
     for (int32_t head = 0; head < heads; ++head) {
@@ -244,15 +271,15 @@ cudaError_t rotary(const fuse_b200_rotary_params& p, cudaStream_t stream) {
   if (p.kv_heads > 0)
     vectors = vectors && host::aligned16(p.k) && host::aligned16(p.k_output) && a.k_stride % 8 == 0 && a.ko_stride % 8 == 0;
   if (vectors) {
-    // rows per block: about 1024 items (four per thread), while the angles stay within 32 KiB
-    const int64_t per_row = int64_t(p.q_heads + p.kv_heads) * (d / 16);
-    int32_t tokens = int32_t(per_row >= 1024 ? 1 : 1024 / per_row);
-    if (tokens > 32) tokens = 32;
+    // rows per block: one batch of every thread, while the angles stay within 24 KiB
+    const int64_t slots = int64_t(p.q_heads + p.kv_heads) * (d / 16);
+    int64_t tokens = slots < kBlock ? kBatch * (kBlock / slots) : kBatch;
+    if (tokens * (n / 2) > 3072) tokens = 3072 / (n / 2);
     const int64_t chunks = (p.rows + tokens - 1) / tokens, resident = int64_t(info.sm_count) * 8;
     const unsigned grid = unsigned(chunks < resident ? chunks : resident);
     const size_t shared = size_t(tokens) * (n / 2) * sizeof(float2);
-    if (p.spec.interleaved) rotary_kernel<true><<<grid, 256, shared, stream>>>(a, tokens);
-    else rotary_kernel<false><<<grid, 256, shared, stream>>>(a, tokens);
+    if (p.spec.interleaved) rotary_kernel<true><<<grid, kBlock, shared, stream>>>(a, int32_t(tokens));
+    else rotary_kernel<false><<<grid, kBlock, shared, stream>>>(a, int32_t(tokens));
   } else {
     const int64_t threads = p.rows * (n / 2 + (d - n));
     const int64_t blocks = (threads + 255) / 256, resident = int64_t(info.sm_count) * 8;
