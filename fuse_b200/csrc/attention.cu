@@ -171,30 +171,39 @@ size_t delta_bytes(const fuse_b200_attention_params& p) {
 // further block costs its FP32 partial sums (128 KiB written and read with heads of 128); shorter than eight
 // tiles, a block's set-up shows.
 struct ChunkPlan {
-  int32_t chunk, max_chunks, key_tiles;
+  int32_t chunk, key_tiles, long_tiles, long_chunks, short_chunks;
+  int64_t sequence_chunks, partial_chunks;
   size_t partial_bytes;
 };
 ChunkPlan plan_chunks(const fuse_b200_attention_params& p, int sm_count) {
   const int32_t pack = packed_heads(p), tokens = attn::kTile / pack, packs = p.q_heads / p.kv_heads / pack;
   ChunkPlan plan{};
   plan.key_tiles = (p.kv_len + attn::kTile - 1) / attn::kTile;
-  const int64_t longest = int64_t((p.q_len + tokens - 1) / tokens) * packs;  // every query tile
-  double seen = double(longest);
+  plan.long_tiles = plan.key_tiles;
+  const int64_t token_tiles = (int64_t(p.q_len) + tokens - 1) / tokens, longest = token_tiles * packs;  // every query tile
+  int64_t usual = longest;  // of a key tile without sinks, at most
+  double total = double(longest) * plan.key_tiles;
   if (p.causal && p.window > 0 && p.window < p.kv_len) {
-    const double window = double((int64_t(p.window) + attn::kTile) / tokens + 1) * packs;
-    if (window < seen) seen = window;
+    // its queries' positions span 127 + window at most
+    const int64_t near = (int64_t(p.window) + attn::kTile - 1 + tokens - 1) / tokens + 1;
+    if (near < token_tiles) usual = near * packs;
+    const int64_t sinks = (int64_t(p.sinks) + attn::kTile - 1) / attn::kTile;
+    plan.long_tiles = int32_t(sinks < plan.key_tiles ? sinks : plan.key_tiles);
+    total = double(longest) * plan.long_tiles + double(usual) * (plan.key_tiles - plan.long_tiles);
   } else if (p.causal && p.kv_len < 2 * int64_t(p.q_len)) {
-    seen *= 0.5;  // (of the keys that are queries' own; those before are seen by all)
+    total *= 0.5;  // (of the keys that are queries' own; those before are seen by all)
   }
-  const double total = seen * plan.key_tiles * p.kv_heads * p.batch;
+  total *= double(p.kv_heads) * p.batch;
   int64_t chunk = int64_t(std::ceil(total / (2.0 * sm_count)));
   if (chunk < 8) chunk = 8;
   if (chunk > longest) chunk = longest > 0 ? longest : 1;
   plan.chunk = int32_t(chunk);
-  plan.max_chunks = int32_t((longest + chunk - 1) / chunk);
-  if (plan.max_chunks < 1) plan.max_chunks = 1;
-  if (plan.max_chunks > 1)
-    plan.partial_bytes = size_t(plan.key_tiles) * p.kv_heads * p.batch * plan.max_chunks * 2 * attn::kTile * p.head_dim * sizeof(float);
+  plan.long_chunks = int32_t(longest > chunk ? (longest + chunk - 1) / chunk : 1);
+  plan.short_chunks = int32_t(usual > chunk ? (usual + chunk - 1) / chunk : 1);
+  const int64_t of_long = int64_t(plan.long_tiles) * plan.long_chunks;
+  plan.sequence_chunks = of_long + int64_t(plan.key_tiles - plan.long_tiles) * plan.short_chunks;
+  plan.partial_chunks = plan.short_chunks > 1 ? plan.sequence_chunks : plan.long_chunks > 1 ? of_long : 0;
+  plan.partial_bytes = size_t(plan.partial_chunks) * p.kv_heads * p.batch * 2 * attn::kTile * p.head_dim * sizeof(float);
   return plan;
 }
 
@@ -209,7 +218,7 @@ cudaError_t backward_workspace_size(const fuse_b200_attention_backward_params& p
 
 template <int kDim>
 cudaError_t launch_backward(const fuse_b200_attention_params& p, const attn::BackwardArgs& b, int64_t q_stride,
-                            int64_t k_stride, int64_t v_stride, cudaStream_t stream) {
+                            int64_t k_stride, int64_t v_stride, int64_t sequence_chunks, cudaStream_t stream) {
   CUtensorMap q, d_o, k, v;
   cudaError_t status;
   const attn::Args& a = b.f;
@@ -227,7 +236,8 @@ cudaError_t launch_backward(const fuse_b200_attention_params& p, const attn::Bac
                                               attn::kTile, 1)) != cudaSuccess)
     return status;
   const int64_t query_tiles = (int64_t(p.q_len) + tokens - 1) / tokens * (p.q_heads / a.pack) * p.batch;
-  const int64_t key_tiles = int64_t(b.key_tiles) * p.kv_heads * p.batch, key_blocks = key_tiles * b.max_chunks;
+  const int64_t key_tiles = int64_t(b.key_tiles) * p.kv_heads * p.batch;
+  const int64_t key_blocks = sequence_chunks * p.kv_heads * p.batch;
   if (query_tiles > INT32_MAX || key_blocks > INT32_MAX) return cudaErrorInvalidValue;
   if (query_tiles > 0 &&
       (status = host::launch_kernel(attn::attention_query_grad_kernel<kDim>, int(query_tiles), attn::kBackwardThreads,
@@ -236,7 +246,7 @@ cudaError_t launch_backward(const fuse_b200_attention_params& p, const attn::Bac
   if (key_tiles == 0) return cudaSuccess;
   status = host::launch_kernel(attn::attention_key_grad_kernel<kDim>, int(key_blocks), attn::kBackwardThreads,
                                attn::KeyGradLayout<kDim>::kDynamicBytes, false, stream, q, d_o, k, v, b);
-  if (status != cudaSuccess || b.max_chunks == 1) return status;
+  if (status != cudaSuccess || b.partial_chunks == 0) return status;
   attn::attention_key_grad_join_kernel<kDim><<<dim3(unsigned(key_tiles), key_tiles < 592 ? 8 : 2), 256, 0, stream>>>(b);
   status = cudaGetLastError();
   if (status == cudaSuccess) host::count_launch();
@@ -272,8 +282,12 @@ cudaError_t attention_backward(const fuse_b200_attention_backward_params& g, con
   const ChunkPlan plan = plan_chunks(p, info.sm_count);
   if (g.workspace_bytes < delta_bytes(p) + plan.partial_bytes) return cudaErrorInvalidValue;
   b.chunk = plan.chunk;
-  b.max_chunks = plan.max_chunks;
   b.key_tiles = plan.key_tiles;
+  b.long_tiles = plan.long_tiles;
+  b.long_chunks = plan.long_chunks;
+  b.short_chunks = plan.short_chunks;
+  if (plan.sequence_chunks > INT32_MAX) return cudaErrorInvalidValue;
+  b.partial_chunks = int32_t(plan.partial_chunks);
   b.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(g.workspace) + delta_bytes(p));
   b.o = p.output;
   b.d_o = g.grad_output;
@@ -283,8 +297,8 @@ cudaError_t attention_backward(const fuse_b200_attention_backward_params& g, con
   b.dk = g.grad_k;
   b.dv = g.grad_v;
   b.f.wait = host::make_wait(info, 0, options ? options->wait_budget_ns : 0);
-  return p.head_dim == 128 ? launch_backward<128>(p, b, q_stride, k_stride, v_stride, stream)
-                           : launch_backward<64>(p, b, q_stride, k_stride, v_stride, stream);
+  return p.head_dim == 128 ? launch_backward<128>(p, b, q_stride, k_stride, v_stride, plan.sequence_chunks, stream)
+                           : launch_backward<64>(p, b, q_stride, k_stride, v_stride, plan.sequence_chunks, stream);
 }
 
 }  // namespace

@@ -29,9 +29,17 @@ struct BackwardArgs {
   float* delta;  // [q_heads][q_rows]
   uint16_t *dq, *dk, *dv;
   int64_t dq_stride, dk_stride, dv_stride;
-  // the key gradients of a key tile that more than `chunk` query tiles see are made by several blocks
-  int32_t chunk, max_chunks, key_tiles;
-  float* partial;  // [batch][kv head][key tile][max_chunks][dV, dK][128][head_dim]
+  // The key gradients of a key tile that more than `chunk` query tiles see are made by several blocks.  The first
+  // `long_tiles` key tiles of a sequence (all, or those with sinks where a window limits the others) have room for
+  // `long_chunks` of them, the others for `short_chunks`.
+  int32_t chunk, key_tiles, long_tiles, long_chunks, short_chunks;
+  int32_t partial_chunks;  // of one sequence: all of its chunks, or none behind the long tiles' where those are alone
+  float* partial;          // [batch][kv head][partial_chunks][dV, dK][128][head_dim]
+  // chunk 0 of a key tile among the sequence's, and from one chunk to the next
+  __device__ __forceinline__ int32_t first_chunk(int32_t tile) const {
+    return tile < long_tiles ? tile : long_tiles * long_chunks + tile - long_tiles;
+  }
+  __device__ __forceinline__ int32_t chunk_step(int32_t tile) const { return tile < long_tiles ? long_tiles : key_tiles - long_tiles; }
 };
 
 constexpr int kBackwardThreads = 384, kElementwiseThreads = 256;
@@ -379,9 +387,10 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   int32_t at = int32_t(blockIdx.x);
   const int32_t kv_head = at % a.kv_heads;
   at /= a.kv_heads;
-  const int32_t b = at % a.batch;
-  at /= a.batch;
-  const int32_t key_tile = at % ba.key_tiles, chunk = at / ba.key_tiles, k0 = key_tile * kTile;
+  const int32_t b = at % a.batch, slot = at / a.batch;
+  const bool is_long = slot < ba.long_tiles * ba.long_chunks;
+  const int32_t among = is_long ? slot : slot - ba.long_tiles * ba.long_chunks, tiles_alike = is_long ? ba.long_tiles : ba.key_tiles - ba.long_tiles;
+  const int32_t chunk = among / tiles_alike, key_tile = among - chunk * tiles_alike + (is_long ? 0 : ba.long_tiles), k0 = key_tile * kTile;
   const Sequence seq = sequence(a, b);
   if (k0 >= seq.kl) return;
   const QueryTiles tiles(a, seq, key_tile, tile_tokens);
@@ -644,8 +653,8 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             }
             if (!mine) continue;
             if (chunks > 1) {
-              const int64_t slot = ((int64_t(b) * a.kv_heads + kv_head) * ba.key_tiles + key_tile) * ba.max_chunks + chunk;
-              uint4* to4 = reinterpret_cast<uint4*>(ba.partial + ((slot * 2 + which) * kTile + row) * kDim + column);
+              const int64_t place = (int64_t(b) * a.kv_heads + kv_head) * ba.partial_chunks + slot;
+              uint4* to4 = reinterpret_cast<uint4*>(ba.partial + ((place * 2 + which) * kTile + row) * kDim + column);
 #pragma unroll
               for (int i = 0; i < 8; ++i) to4[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             } else {
@@ -682,15 +691,16 @@ __global__ void __launch_bounds__(256) attention_key_grad_join_kernel(const __gr
   const int32_t all = QueryTiles(a, seq, key_tile, kTile >> a.pack_shift).count * ((a.q_heads / a.kv_heads) >> a.pack_shift);
   const int32_t chunks = (all + ba.chunk - 1) / ba.chunk;
   if (chunks <= 1) return;
-  const int64_t slot = ((int64_t(b) * a.kv_heads + kv_head) * ba.key_tiles + key_tile) * ba.max_chunks;
+  const int64_t place = (int64_t(b) * a.kv_heads + kv_head) * ba.partial_chunks + ba.first_chunk(key_tile);
+  const int64_t step = int64_t(ba.chunk_step(key_tile)) * 2 * kTile * kDim;
   const int32_t rows = min(kTile, seq.kl - k0);
   constexpr int kVectors = kDim / 4;
   for (int32_t i = int32_t(blockIdx.y) * 256 + threadIdx.x; i < 2 * rows * kVectors; i += int32_t(gridDim.y) * 256) {
     const int32_t which = i / (rows * kVectors), rest = i - which * rows * kVectors, row = rest / kVectors, column = rest % kVectors * 4;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float* from = ba.partial + ((slot * 2 + which) * kTile + row) * kDim + column;
+    const float* from = ba.partial + ((place * 2 + which) * kTile + row) * kDim + column;
     for (int32_t c = 0; c < chunks; ++c) {
-      const float4 v = *reinterpret_cast<const float4*>(from + int64_t(c) * 2 * kTile * kDim);
+      const float4 v = *reinterpret_cast<const float4*>(from + c * step);
       sum.x += v.x;
       sum.y += v.y;
       sum.z += v.z;

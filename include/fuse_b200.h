@@ -560,7 +560,7 @@ FUSE_API int fuse_launch_oproj_backward_mxfp8(const fuse_mxfp8_oproj_backward_pa
 /* h = bf16(input + residual);  y = h * rsqrt(mean(h^2) + epsilon) * gamma, the mean in FP32.
  * hidden: a multiple of 8 (of 32 with `quantized`), at most 16384; epsilon at least 1e-30.  Strides:
  * multiples of 8, pointers 16-byte aligned.  `residual` may be NULL; `residual_output` receives h and may be NULL, or `input` or
- * `residual` themselves.  `output` receives bf16(y), `quantized` the MXFP8 form of that BF16 tensor
+ * `residual` themselves (so may `output`, with the same stride).  `output` receives bf16(y), `quantized` the MXFP8 form of that BF16 tensor
  * (E4M3 [rows, hidden] packed, scales in native atoms, 2^0 where an atom reaches past the operand):
  * the same bytes fuse_b200_quantize_mxfp8 makes of `output`.  One of the two at least. */
 typedef struct fuse_b200_rms_norm_params {
@@ -663,7 +663,7 @@ FUSE_API int fuse_b200_launch_rotary(const fuse_b200_rotary_params* params, fuse
  * infinity in a key or value of the sequence itself may reach queries that do not see it.
  *
  * `lse` (may be NULL): FP32 [q_heads][q_rows], log of the sum of exp(scale q k) -- what the backward needs.
- * `workspace` (256-byte aligned, fuse_b200_attention_workspace_size; may be 0 bytes) holds partial results when
+ * `output` must not overlap an input.  `workspace` (256-byte aligned, fuse_b200_attention_workspace_size; may be 0 bytes) holds partial results when
  * the keys are split because the queries alone would leave SMs idle; two launches that may run at the same
  * time need two. */
 typedef struct fuse_b200_attention_params {
@@ -689,7 +689,8 @@ FUSE_API int fuse_b200_launch_attention(const fuse_b200_attention_params* params
 
 /* Gradients of the above.  `forward`: the forward's record, with its output and lse as inputs (its workspace is not
  * used).  grad_q like q, grad_k and grad_v like k: rows of the sequences are written, others left as they
- * were; none of them may overlap an input.  No atomics: the same inputs give the same bits.
+ * were; none of them may overlap an input.  q_rows must not be 0 where kv_rows is not, and sequences must not share
+ * rows (the forward alone may read the same keys for several).  No atomics: the same inputs give the same bits.
  * workspace: 256-byte aligned, fuse_b200_attention_backward_workspace_size bytes. */
 typedef struct fuse_b200_attention_backward_params {
   fuse_b200_attention_params forward;

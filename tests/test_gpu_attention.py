@@ -286,3 +286,48 @@ def test_refusals():
                  lambda: block.attention(q.clone().requires_grad_(), k, v, head_dim=64, out=torch.empty_like(q))):
         with pytest.raises(RuntimeError):
             call()
+
+
+# key tiles that many query tiles see are made in chunks: all (causal, few KV heads), or those with sinks
+@pytest.mark.parametrize("kw", [dict(), dict(window=200, sinks=150), dict(window=40, sinks=1), dict(causal=False), dict(window=900, sinks=0)])
+@pytest.mark.parametrize("shape", [(1, 1500, 1500, 8, 1, 64), (2, 900, 1100, 6, 2, 128)])
+def test_key_gradients_in_chunks(kw, shape):
+    b, ql, kl, hq, hk, d = shape
+    run_all(*make(b * ql, b * kl, hq, hk, d, 111), head_dim=d, batch=b, **kw)
+
+
+def test_workspace_of_a_long_context_stays_small():
+    p = N.AttentionBackwardParams(forward=N.AttentionParams(
+        q_rows=1 << 19, kv_rows=1 << 19, batch=1, q_len=1 << 19, kv_len=1 << 19, q_heads=8, kv_heads=1, head_dim=128, causal=1,
+        window=4096, sinks=4, scale=1.0))
+    rc, size = api.attention_backward_workspace_size(p)
+    assert rc == 0 and size < 1 << 27
+    p.forward.window = 0
+    rc, size = api.attention_backward_workspace_size(p)
+    assert rc == 0 and size < 1 << 27
+    p.forward.q_len = p.forward.kv_len = p.forward.q_rows = p.forward.kv_rows = 25600
+    p.forward.window = 128
+    rc, size = api.attention_backward_workspace_size(p)
+    assert rc == 0 and size < 1 << 28
+
+
+def test_shared_keys_without_gradients():
+    q, k, v, _ = make(3 * 20, 500, 4, 2, 64, 121)
+    out = block.attention(q, k, v, head_dim=64, batch=3, kv_len=500, kv_starts=i32(0, 0, 100), kv_lengths=i32(500, 300, 300))
+    for i, (s, n) in enumerate(((0, 500), (0, 300), (100, 300))):
+        want = attention64(q[20 * i:20 * i + 20], k[s:s + n], v[s:s + n], head_dim=64)
+        check({"o": out[20 * i:20 * i + 20]}, want, ["o"])
+
+
+def test_no_queries_and_no_keys():
+    q, k, v, _ = make(0, 64, 2, 1, 64, 131)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = block.attention(*leaves, head_dim=64)
+    assert out.shape == (0, 128)
+    dq, dk, dv = torch.autograd.grad(out, leaves, torch.zeros_like(out))
+    assert dq.shape == (0, 128) and (dk == 0).all() and (dv == 0).all()
+    q, k, v, do = make(40, 64, 2, 1, 64, 132)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out, lse = block.attention(*leaves, head_dim=64, kv_lengths=i32(0), return_lse=True)
+    assert (out == 0).all() and torch.isinf(lse).all()
+    assert all((g == 0).all() for g in torch.autograd.grad(out, leaves, do))

@@ -214,3 +214,23 @@ def test_captured_and_on_another_stream():
     want_y, want_h = block.rms_norm(fresh, gamma, res)
     want_dx, = torch.autograd.grad((want_y, want_h), fresh, (dy, dh))
     assert torch.equal(y, want_y) and torch.equal(dx, want_dx)
+
+
+def test_backward_of_no_rows():
+    x, gamma = torch.empty(0, 512, dtype=BF16, device=DEV, requires_grad=True), torch.ones(512, dtype=BF16, device=DEV, requires_grad=True)
+    y, h = block.rms_norm(x, gamma)
+    dx, dgamma = torch.autograd.grad(y, (x, gamma), torch.empty_like(y))
+    assert dx.shape == (0, 512) and (dgamma == 0).all()
+
+
+def test_gradients_past_the_range_of_fp32_squares():
+    x, _, gamma, dy, _ = make(5, 640, 17, 1e25)
+    x = x.requires_grad_()
+    y, _ = block.rms_norm(x, gamma)
+    dx, = torch.autograd.grad(y, x, dy)
+    h, d = x.detach().double(), dy.double() * gamma.double()
+    r = torch.rsqrt(h.square().mean(1, keepdim=True) + EPS)
+    n = h * r
+    want = r * (d - n * (d * n).mean(1, keepdim=True))
+    size = r * (d.abs() + n.abs() * (d * n).abs().mean(1, keepdim=True))
+    within(dx, want, want.abs() * 2.0 ** -8 + size * 2.0 ** -16 + 2.0 ** -134, "dx")
