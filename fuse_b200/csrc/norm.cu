@@ -31,6 +31,7 @@ struct NormGradArgs {
   const uint16_t *dy, *h, *gamma, *dh;
   uint16_t* dx;
   float* partial;  // [row groups of the grid][hidden], or nullptr
+  WaitContext wait;
   int64_t dy_stride, h_stride, dh_stride, dx_stride, rows;
   int32_t hidden;
   float eps;
@@ -188,13 +189,122 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kern
   }
 }
 
-// Backward of one row per step; the block keeps its rows' share of the gamma gradient in registers and
-// writes it as one row of `partial`.
-template <int kThreads, int kVec>
-__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_backward_kernel(const NormGradArgs a) {
-  constexpr int kBlock = kThreads < 128 ? 128 : kThreads, kRows = kBlock / kThreads;
-  __shared__ float scratch[2 * (kBlock / 32) * 2];
-  const int t = threadIdx.x % kThreads;
+// The row's share of both outputs, from its vectors j of kThreads * 8 elements.
+__device__ __forceinline__ void grad_vector(const uint4& h, const uint4& dy, const uint4& gamma, const uint4& dh, float r, float mean,
+                                            float (&acc)[8], uint16_t* to) {
+  float fh[8], fd[8], fg[8], out[8];
+  unpack8(h, fh);
+  unpack8(dy, fd);
+  unpack8(gamma, fg);
+  unpack8(dh, out);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float n = fh[i] * r;
+    acc[i] = fmaf(fd[i], n, acc[i]);
+    out[i] = fmaf(r, fmaf(fd[i], fg[i], -n * mean), out[i]);
+  }
+  *reinterpret_cast<uint4*>(to) = pack8(out);
+}
+// What a vector adds to the sums of h^2 and of dy g h, h scaled by `down`.
+__device__ __forceinline__ void grad_sums(const uint4& h, const uint4& dy, const uint4& gamma, float down, float (&sum)[2]) {
+  float fh[8], fd[8], fg[8];
+  unpack8(h, fh);
+  unpack8(dy, fd);
+  unpack8(gamma, fg);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = fh[i] * down;
+    sum[0] = fmaf(x, x, sum[0]);
+    sum[1] = fmaf(fd[i] * fg[i], x, sum[1]);
+  }
+}
+__device__ __forceinline__ void store_share(const float (&acc)[8], float* to) {
+  reinterpret_cast<float4*>(to)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  reinterpret_cast<float4*>(to)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+}
+
+// Backward, a warp per row (hidden up to 512): the row stays in registers, as does the warp's share of the gamma
+// gradient, which it writes as one row of `partial`.
+template <int kVec>
+__global__ void __launch_bounds__(128) rms_norm_backward_warp_kernel(const NormGradArgs a) {
+  const int t = threadIdx.x & 31;
+  uint4 gamma[kVec];
+  float acc[kVec][8];
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    const int32_t c = (j * 32 + t) * 8;
+    gamma[j] = c < a.hidden ? load16(a.gamma + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
+  }
+  const float inv = 1.0f / float(a.hidden);
+  const int64_t group = int64_t(blockIdx.x) * 4 + threadIdx.x / 32;
+  for (int64_t row = group; row < a.rows; row += int64_t(gridDim.x) * 4) {
+    uint4 h[kVec], dy[kVec], dh[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int32_t c = (j * 32 + t) * 8;
+      h[j] = dy[j] = dh[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (c < a.hidden) {
+        h[j] = load16(a.h + row * a.h_stride + c);
+        dy[j] = load16(a.dy + row * a.dy_stride + c);
+        if (a.dh != nullptr) dh[j] = load16(a.dh + row * a.dh_stride + c);
+      }
+    }
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) grad_sums(h[j], dy[j], gamma[j], 1.0f, sum);
+    row_sum<32, 2>(sum, nullptr, 0);
+    float r = rsqrtf(fmaf(sum[0], inv, a.eps)), mean = sum[1] * inv * r;  // mean(dn n)
+    if (!(sum[0] < kTooLarge)) {
+      sum[0] = sum[1] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) grad_sums(h[j], dy[j], gamma[j], kDown, sum);
+      row_sum<32, 2>(sum, nullptr, 0);
+      r = rsqrtf(sum[0] * inv);
+      mean = sum[1] * inv * r;
+      r *= kDown;
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int32_t c = (j * 32 + t) * 8;
+      if (c < a.hidden) grad_vector(h[j], dy[j], gamma[j], dh[j], r, mean, acc[j], a.dx + row * a.dx_stride + c);
+    }
+  }
+  if (a.partial != nullptr) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int32_t c = (j * 32 + t) * 8;
+      if (c < a.hidden) store_share(acc[j], a.partial + group * a.hidden + c);
+    }
+  }
+}
+
+// Backward, a block per row: the three input rows arrive in shared memory by bulk copies, two rows of the block's walk
+// in flight, so that loads go on across the row's two barriers.
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const NormGradArgs a) {
+  constexpr int kVec = 4, kStages = 2;
+  extern __shared__ __align__(128) uint8_t rows_shared[];  // [kStages][h, dy, dh][hidden]
+  __shared__ float scratch[2 * (kThreads / 32) * 2];
+  __shared__ __align__(8) uint64_t bars[kStages];
+  const int t = threadIdx.x;
+  const uint32_t row_bytes = uint32_t(a.hidden) * 2, inputs = a.dh != nullptr ? 3u : 2u;
+  const uint32_t base = ptx::smem_u32(rows_shared);
+  auto bar = [&](int s) { return ptx::smem_u32(bars + s); };
+  auto fetch = [&](int s, int64_t row) {  // one thread
+    const uint32_t to = base + uint32_t(s) * 3 * row_bytes;
+    ptx::mbar_expect_tx(bar(s), inputs * row_bytes);
+    ptx::bulk_load(to, a.h + row * a.h_stride, row_bytes, bar(s));
+    ptx::bulk_load(to + row_bytes, a.dy + row * a.dy_stride, row_bytes, bar(s));
+    if (a.dh != nullptr) ptx::bulk_load(to + 2 * row_bytes, a.dh + row * a.dh_stride, row_bytes, bar(s));
+  };
+  if (t == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(bar(s), 1);
+    ptx::fence_mbar_init();
+    for (int s = 0; s < kStages; ++s)
+      if (blockIdx.x + int64_t(s) * gridDim.x < a.rows) fetch(s, blockIdx.x + int64_t(s) * gridDim.x);
+  }
   uint4 gamma[kVec];
   float acc[kVec][8];
 #pragma unroll
@@ -204,51 +314,32 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_back
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
   }
+  __syncthreads();
   const float inv = 1.0f / float(a.hidden);
-  const int64_t group = int64_t(blockIdx.x) * kRows + threadIdx.x / kThreads;
-  int slot = 0;
-  for (int64_t row = group; row < a.rows; row += int64_t(gridDim.x) * kRows) {
-    uint4 h[kVec], dy[kVec], dh[kVec];
+  int slot = 0, stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    // the block decides together whether the row has come
+    ok = __syncthreads_and(mbar_wait(bar(stage), phase, a.wait, kSiteSmemFull)) != 0;
+    if (!ok) break;
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(rows_shared) + int64_t(stage) * 3 * a.hidden;
+    const uint16_t *dy = h + a.hidden, *dh = dy + a.hidden;
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int32_t c = (j * kThreads + t) * 8;
-      h[j] = dy[j] = dh[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (c < a.hidden) {
-        h[j] = load16(a.h + row * a.h_stride + c);
-        dy[j] = load16(a.dy + row * a.dy_stride + c);
-        if (a.dh != nullptr) dh[j] = load16(a.dh + row * a.dh_stride + c);
-      }
-    }
-    float sum[2] = {0.0f, 0.0f};  // of h^2 and of dy g h
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      float fh[8], fd[8], fg[8];
-      unpack8(h[j], fh);
-      unpack8(dy[j], fd);
-      unpack8(gamma[j], fg);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum[0] = fmaf(fh[i], fh[i], sum[0]);
-        sum[1] = fmaf(fd[i] * fg[i], fh[i], sum[1]);
-      }
+      if (c < a.hidden) grad_sums(load16(h + c), load16(dy + c), gamma[j], 1.0f, sum);
     }
     row_sum<kThreads, 2>(sum, scratch, slot);
     slot ^= 1;
-    float r = rsqrtf(fmaf(sum[0], inv, a.eps));
-    float mean = sum[1] * inv * r;  // mean(dn n)
+    float r = rsqrtf(fmaf(sum[0], inv, a.eps)), mean = sum[1] * inv * r;  // mean(dn n)
     if (!(sum[0] < kTooLarge)) {
       sum[0] = sum[1] = 0.0f;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        float fh[8], fd[8], fg[8];
-        unpack8(h[j], fh);
-        unpack8(dy[j], fd);
-        unpack8(gamma[j], fg);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          sum[0] = fmaf(fh[i] * kDown, fh[i] * kDown, sum[0]);
-          sum[1] = fmaf(fd[i] * fg[i], fh[i] * kDown, sum[1]);
-        }
+        const int32_t c = (j * kThreads + t) * 8;
+        if (c < a.hidden) grad_sums(load16(h + c), load16(dy + c), gamma[j], kDown, sum);
       }
       row_sum<kThreads, 2>(sum, scratch, slot);
       slot ^= 1;
@@ -259,29 +350,27 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_back
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int32_t c = (j * kThreads + t) * 8;
-      float fh[8], fd[8], fg[8], out[8];
-      unpack8(h[j], fh);
-      unpack8(dy[j], fd);
-      unpack8(gamma[j], fg);
-      unpack8(dh[j], out);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float n = fh[i] * r;
-        acc[j][i] = fmaf(fd[i], n, acc[j][i]);
-        out[i] = fmaf(r, fmaf(fd[i], fg[i], -n * mean), out[i]);
-      }
-      if (c < a.hidden) *reinterpret_cast<uint4*>(a.dx + row * a.dx_stride + c) = pack8(out);
+      if (c < a.hidden)
+        grad_vector(load16(h + c), load16(dy + c), gamma[j], a.dh != nullptr ? load16(dh + c) : make_uint4(0u, 0u, 0u, 0u), r, mean,
+                    acc[j], a.dx + row * a.dx_stride + c);
     }
+    __syncthreads();  // the stage is read
+    if (t == 0 && row + int64_t(kStages) * gridDim.x < a.rows) fetch(stage, row + int64_t(kStages) * gridDim.x);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  if (!ok) {  // a wait gave up: copies in flight get their time to land before shared memory goes away
+    const uint64_t start = ptx::globaltimer();
+    while (ptx::globaltimer() - start < 200000ull) __nanosleep(1000);
+    return;
   }
   if (a.partial != nullptr) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int32_t c = (j * kThreads + t) * 8;
-      if (c < a.hidden) {
-        float4* to = reinterpret_cast<float4*>(a.partial + group * a.hidden + c);
-        to[0] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-        to[1] = make_float4(acc[j][4], acc[j][5], acc[j][6], acc[j][7]);
-      }
+      if (c < a.hidden) store_share(acc[j], a.partial + int64_t(blockIdx.x) * a.hidden + c);
     }
   }
 }
@@ -310,10 +399,15 @@ constexpr int32_t kMaxHidden = 16384;
 // Threads of a row: as few as hold it in four vectors each; a warp (no block barrier, four rows to a
 // block) or whole blocks of 128 and more.
 int row_threads(int32_t hidden) { return hidden <= 1024 ? 32 : hidden <= 4096 ? 128 : hidden <= 8192 ? 256 : 512; }
-// Row groups of the backward grid (rows of `partial`): whole blocks, as many as stay resident.
+// The backward's: a warp as far as its registers hold the row and its gradients without thinning the SM out.
+int grad_threads(int32_t hidden) { return hidden <= 512 ? 32 : row_threads(hidden < 4096 ? 4096 : hidden); }
+// Row groups of the backward grid (rows of `partial`): whole blocks, as many as stay resident.  A block per row keeps two
+// rows of three inputs in shared memory (6 bytes per element and row) and 512 threads fill an SM's registers.
 int backward_groups(int64_t rows, int32_t hidden, int sm_count) {
-  const int threads = row_threads(hidden), block = threads < 128 ? 128 : threads, per_block = block / threads;
-  const int64_t resident = int64_t(sm_count) * (512 / block);
+  const int threads = grad_threads(hidden), block = threads < 128 ? 128 : threads, per_block = block / threads;
+  int64_t per_sm = 512 / block;
+  if (threads >= 128 && per_sm * 12 * hidden > 200 * 1024) per_sm = 200 * 1024 / (12 * hidden);
+  const int64_t resident = int64_t(sm_count) * (per_sm > 0 ? per_sm : 1);
   const int64_t wanted = (rows + per_block - 1) / per_block;
   return int((wanted < resident ? wanted : resident) * per_block);
 }
@@ -412,7 +506,7 @@ cudaError_t rms_norm_backward(const fuse_b200_rms_norm_backward_params& p, cudaS
   DeviceInfo info;
   cudaError_t status = launch::check_device(&info);
   if (status != cudaSuccess) return status;
-  const int threads = row_threads(p.hidden), block = threads < 128 ? 128 : threads;
+  const int threads = grad_threads(p.hidden), block = threads < 128 ? 128 : threads;
   const int groups = backward_groups(p.rows, p.hidden, info.sm_count);
   const unsigned grid = unsigned(groups / (block / threads));
   if (p.grad_gamma != nullptr && groups > 0 &&
@@ -425,20 +519,23 @@ cudaError_t rms_norm_backward(const fuse_b200_rms_norm_backward_params& p, cudaS
   a.dh = p.grad_stream;
   a.dx = p.grad_input;
   a.partial = p.grad_gamma != nullptr ? static_cast<float*>(p.workspace) : nullptr;
+  a.wait = host::make_wait(info, 0, 0);
   if (grid > 0) {
     const int vec = (p.hidden + threads * 8 - 1) / (threads * 8);
-    switch (threads) {
-      case 32:
-        if (vec == 1) rms_norm_backward_kernel<32, 1><<<grid, block, 0, stream>>>(a);
-        else if (vec == 2) rms_norm_backward_kernel<32, 2><<<grid, block, 0, stream>>>(a);
-        else rms_norm_backward_kernel<32, 4><<<grid, block, 0, stream>>>(a);
-        break;
-      case 128: rms_norm_backward_kernel<128, 4><<<grid, block, 0, stream>>>(a); break;
-      case 256: rms_norm_backward_kernel<256, 4><<<grid, block, 0, stream>>>(a); break;
-      default: rms_norm_backward_kernel<512, 4><<<grid, block, 0, stream>>>(a); break;
+    const uint32_t shared = uint32_t(2 * 3 * 2 * p.hidden);
+    if (threads == 128) {
+      status = host::launch_kernel(rms_norm_backward_kernel<128>, int(grid), 128, shared, false, stream, a);
+    } else if (threads == 256) {
+      status = host::launch_kernel(rms_norm_backward_kernel<256>, int(grid), 256, shared, false, stream, a);
+    } else if (threads == 512) {
+      status = host::launch_kernel(rms_norm_backward_kernel<512>, int(grid), 512, shared, false, stream, a);
+    } else {
+      if (vec == 1) rms_norm_backward_warp_kernel<1><<<grid, 128, 0, stream>>>(a);
+      else rms_norm_backward_warp_kernel<2><<<grid, 128, 0, stream>>>(a);
+      status = cudaGetLastError();
+      if (status == cudaSuccess) host::count_launch();
     }
-    if ((status = cudaGetLastError()) != cudaSuccess) return status;
-    host::count_launch();
+    if (status != cudaSuccess) return status;
   }
   if (p.grad_gamma != nullptr) {
     rms_norm_gamma_kernel<<<unsigned((p.hidden + 31) / 32), 1024, 0, stream>>>(a.partial, groups, p.hidden, p.grad_gamma);
