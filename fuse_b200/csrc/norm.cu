@@ -8,9 +8,11 @@
 // which is by definition the quantisation of the BF16 output (so that a caller may mix the two).
 //
 // Bound by HBM: the forward moves 8 bytes per element (7.03 with MXFP8 out), the backward 8.  A row
-// stays in registers between its sum and its scaling, so every element is read once.  A row belongs to
-// a warp or to a block of 128 to 512 threads (16-byte vectors, at most four per thread); blocks walk the rows with the grid's
-// stride and keep gamma in registers.
+// stays in registers between its sum and its scaling, so every element is read once; it belongs to a warp
+// or to a block (16-byte vectors, two to four per thread: with four in the forward the registers thin
+// the SM out, 16384 x 4096 to MXFP8 100 us against 91).  The backward of wide rows stages them in shared memory instead.
+// Blocks walk the rows with the grid's stride and keep gamma in registers.  Measured: forward 8191 x 8192 80 us (6.7 TB/s), backward
+// 82 us (6.6) and 6 for the join of dgamma; 16384 x 4096 to MXFP8 91 us (5.2 TB/s: conversions and scale words share the issue slots).
 #include "launch.cuh"
 
 namespace fuse_b200 {
@@ -55,25 +57,27 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// Sum over the kThreads threads of one row; `slot` alternates from row to row, so that one barrier per
+constexpr int kVectors = 2;                // of a thread in a block per row
+constexpr int kMaxWarps = 64 / kVectors;  // of a block, which has one row
+
+// Sum over the threads of one row, a warp or the block; `slot` alternates from row to row, so that one barrier per
 // row is enough (a slot is written again only after the barrier of the row in between).
-template <int kThreads, int kValues>
+template <bool kWarpRow, int kValues>
 __device__ __forceinline__ void row_sum(float (&v)[kValues], float* scratch, int slot) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < kValues; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if constexpr (kThreads > 32) {
-    constexpr int kWarps = kThreads / 32;
-    float* mine = scratch + slot * kWarps * kValues;
+  if constexpr (!kWarpRow) {
+    const int warps = int(blockDim.x) >> 5;
+    float* mine = scratch + slot * kMaxWarps * kValues;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int i = 0; i < kValues; ++i) mine[(threadIdx.x >> 5) * kValues + i] = v[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kValues; ++i) v[i] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
+    for (int w = 0; w < warps; ++w)
 #pragma unroll
       for (int i = 0; i < kValues; ++i) v[i] += mine[w * kValues + i];
   }
@@ -85,16 +89,16 @@ constexpr float kTooLarge = 1.7014118e38f;           // 2^127
 constexpr float kDown = 2.1175823681357508e-22f;     // 2^-72
 constexpr float kMinEpsilon = 1e-30f;
 
-// kThreads threads per row: a block of at least 128 holds one row, a block of warps four.
-template <int kThreads, int kVec, bool kMx>
-__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kernel(const NormArgs a) {
-  constexpr int kBlock = kThreads < 128 ? 128 : kThreads, kRows = kBlock / kThreads;
-  __shared__ float scratch[2 * (kBlock / 32)];
-  const int t = threadIdx.x % kThreads;
+// A warp per row (four rows to a block), or a block.
+template <bool kWarpRow, int kVec, bool kMx>
+__global__ void __launch_bounds__(kWarpRow ? 128 : 32 * kMaxWarps) rms_norm_kernel(const NormArgs a) {
+  __shared__ float scratch[2 * kMaxWarps];
+  const int threads = kWarpRow ? 32 : int(blockDim.x), rows_of_block = kWarpRow ? 4 : 1;
+  const int t = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
   uint4 gamma[kVec];
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    const int32_t c = (j * kThreads + t) * 8;
+    const int32_t c = (j * threads + t) * 8;
     gamma[j] = c < a.hidden ? load16(a.gamma + c) : make_uint4(0u, 0u, 0u, 0u);
   }
   const float inv = 1.0f / float(a.hidden);
@@ -102,17 +106,17 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kern
   const int64_t last = kMx ? (a.rows + 127) & ~int64_t(127) : a.rows;
   const int64_t k_atoms = (int64_t(a.hidden) + 127) >> 7;
   int slot = 0;
-  for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kThreads; row < last;
-       row += int64_t(gridDim.x) * kRows) {
+  for (int64_t row = int64_t(blockIdx.x) * rows_of_block + (kWarpRow ? threadIdx.x >> 5 : 0); row < last;
+       row += int64_t(gridDim.x) * rows_of_block) {
     if (kMx && row >= a.rows) {  // (the same for all threads of the row)
-      for (int64_t atom = t; atom < k_atoms; atom += kThreads)
+      for (int64_t atom = t; atom < k_atoms; atom += threads)
         *reinterpret_cast<uint32_t*>(a.scales + mxfp8_scale_offset(row, atom << 7, k_atoms)) = 0x7f7f7f7fu;
       continue;
     }
     uint4 h[kVec], res[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int32_t c = (j * kThreads + t) * 8;
+      const int32_t c = (j * threads + t) * 8;
       h[j] = res[j] = make_uint4(0u, 0u, 0u, 0u);
       if (c < a.hidden) {
         h[j] = load16(a.x + row * a.x_stride + c);
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kern
     float sum[1] = {0.0f};
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int32_t c = (j * kThreads + t) * 8;
+      const int32_t c = (j * threads + t) * 8;
       float f[8];
       if (a.res != nullptr) {
         float g[8];
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kern
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[0] = fmaf(f[i], f[i], sum[0]);
     }
-    row_sum<kThreads, 1>(sum, scratch, slot);
+    row_sum<kWarpRow, 1>(sum, scratch, slot);
     slot ^= 1;
     float r = rsqrtf(fmaf(sum[0], inv, a.eps));
     if (!(sum[0] < kTooLarge)) {  // (the same for all threads of the row)
@@ -149,13 +153,13 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kern
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[0] = fmaf(f[i] * kDown, f[i] * kDown, sum[0]);
       }
-      row_sum<kThreads, 1>(sum, scratch, slot);
+      row_sum<kWarpRow, 1>(sum, scratch, slot);
       slot ^= 1;
       r = rsqrtf(sum[0] * inv) * kDown;  // epsilon is far below the last bit
     }
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int32_t c = (j * kThreads + t) * 8;
+      const int32_t c = (j * threads + t) * 8;
       float f[8], g[8];
       unpack8(h[j], f);
       unpack8(gamma[j], g);
@@ -189,7 +193,7 @@ __global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) rms_norm_kern
   }
 }
 
-// The row's share of both outputs, from its vectors j of kThreads * 8 elements.
+// The row's share of both outputs, from one vector of its elements.
 __device__ __forceinline__ void grad_vector(const uint4& h, const uint4& dy, const uint4& gamma, const uint4& dh, float r, float mean,
                                             float (&acc)[8], uint16_t* to) {
   float fh[8], fd[8], fg[8], out[8];
@@ -254,13 +258,13 @@ __global__ void __launch_bounds__(128) rms_norm_backward_warp_kernel(const NormG
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < kVec; ++j) grad_sums(h[j], dy[j], gamma[j], 1.0f, sum);
-    row_sum<32, 2>(sum, nullptr, 0);
+    row_sum<true, 2>(sum, nullptr, 0);
     float r = rsqrtf(fmaf(sum[0], inv, a.eps)), mean = sum[1] * inv * r;  // mean(dn n)
     if (!(sum[0] < kTooLarge)) {
       sum[0] = sum[1] = 0.0f;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) grad_sums(h[j], dy[j], gamma[j], kDown, sum);
-      row_sum<32, 2>(sum, nullptr, 0);
+      row_sum<true, 2>(sum, nullptr, 0);
       r = rsqrtf(sum[0] * inv);
       mean = sum[1] * inv * r;
       r *= kDown;
@@ -282,13 +286,12 @@ __global__ void __launch_bounds__(128) rms_norm_backward_warp_kernel(const NormG
 
 // Backward, a block per row: the three input rows arrive in shared memory by bulk copies, two rows of the block's walk
 // in flight, so that loads go on across the row's two barriers.
-template <int kThreads>
-__global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const NormGradArgs a) {
+__global__ void __launch_bounds__(512) rms_norm_backward_kernel(const NormGradArgs a) {
   constexpr int kVec = 4, kStages = 2;
   extern __shared__ __align__(128) uint8_t rows_shared[];  // [kStages][h, dy, dh][hidden]
-  __shared__ float scratch[2 * (kThreads / 32) * 2];
+  __shared__ float scratch[2 * kMaxWarps * 2];
   __shared__ __align__(8) uint64_t bars[kStages];
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, threads = blockDim.x;
   const uint32_t row_bytes = uint32_t(a.hidden) * 2, inputs = a.dh != nullptr ? 3u : 2u;
   const uint32_t base = ptx::smem_u32(rows_shared);
   auto bar = [&](int s) { return ptx::smem_u32(bars + s); };
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const NormG
   float acc[kVec][8];
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    const int32_t c = (j * kThreads + t) * 8;
+    const int32_t c = (j * threads + t) * 8;
     gamma[j] = c < a.hidden ? load16(a.gamma + c) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
@@ -328,20 +331,20 @@ __global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const NormG
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int32_t c = (j * kThreads + t) * 8;
+      const int32_t c = (j * threads + t) * 8;
       if (c < a.hidden) grad_sums(load16(h + c), load16(dy + c), gamma[j], 1.0f, sum);
     }
-    row_sum<kThreads, 2>(sum, scratch, slot);
+    row_sum<false, 2>(sum, scratch, slot);
     slot ^= 1;
     float r = rsqrtf(fmaf(sum[0], inv, a.eps)), mean = sum[1] * inv * r;  // mean(dn n)
     if (!(sum[0] < kTooLarge)) {
       sum[0] = sum[1] = 0.0f;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const int32_t c = (j * kThreads + t) * 8;
+        const int32_t c = (j * threads + t) * 8;
         if (c < a.hidden) grad_sums(load16(h + c), load16(dy + c), gamma[j], kDown, sum);
       }
-      row_sum<kThreads, 2>(sum, scratch, slot);
+      row_sum<false, 2>(sum, scratch, slot);
       slot ^= 1;
       r = rsqrtf(sum[0] * inv);
       mean = sum[1] * inv * r;
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const NormG
     }
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int32_t c = (j * kThreads + t) * 8;
+      const int32_t c = (j * threads + t) * 8;
       if (c < a.hidden)
         grad_vector(load16(h + c), load16(dy + c), gamma[j], a.dh != nullptr ? load16(dh + c) : make_uint4(0u, 0u, 0u, 0u), r, mean,
                     acc[j], a.dx + row * a.dx_stride + c);
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_backward_kernel(const NormG
   if (a.partial != nullptr) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int32_t c = (j * kThreads + t) * 8;
+      const int32_t c = (j * threads + t) * 8;
       if (c < a.hidden) store_share(acc[j], a.partial + int64_t(blockIdx.x) * a.hidden + c);
     }
   }
@@ -396,11 +399,14 @@ __global__ void __launch_bounds__(1024) rms_norm_gamma_kernel(const float* parti
 
 constexpr int32_t kMaxHidden = 16384;
 
-// Threads of a row: as few as hold it in four vectors each; a warp (no block barrier, four rows to a
-// block) or whole blocks of 128 and more.
-int row_threads(int32_t hidden) { return hidden <= 1024 ? 32 : hidden <= 4096 ? 128 : hidden <= 8192 ? 256 : 512; }
+// Threads of a row: a warp with up to four vectors each (no block barrier, four rows to a block), or a block of as
+// few as hold it in kVectors each.
+int row_threads(int32_t hidden) {
+  const int threads = (hidden + 256 * kVectors - 1) / (256 * kVectors) * 32;
+  return hidden <= 1024 ? 32 : threads < 128 ? 128 : threads;
+}
 // The backward's: a warp as far as its registers hold the row and its gradients without thinning the SM out.
-int grad_threads(int32_t hidden) { return hidden <= 512 ? 32 : row_threads(hidden < 4096 ? 4096 : hidden); }
+int grad_threads(int32_t hidden) { return hidden <= 512 ? 32 : hidden <= 4096 ? 128 : (hidden + 1023) / 1024 * 32; }
 // Row groups of the backward grid (rows of `partial`): whole blocks, as many as stay resident.  A block per row keeps two
 // rows of three inputs in shared memory (6 bytes per element and row) and 512 threads fill an SM's registers.
 int backward_groups(int64_t rows, int32_t hidden, int sm_count) {
@@ -423,16 +429,10 @@ void launch_forward(const NormArgs& a, int sm_count, cudaStream_t stream) {
   const int64_t wanted = (rows + per_block - 1) / per_block, resident = int64_t(sm_count) * (2048 / block);
   const unsigned grid = unsigned(wanted < resident ? wanted : resident);
   const int vec = (a.hidden + threads * 8 - 1) / (threads * 8);
-  switch (threads) {
-    case 32:
-      if (vec == 1) rms_norm_kernel<32, 1, kMx><<<grid, block, 0, stream>>>(a);
-      else if (vec == 2) rms_norm_kernel<32, 2, kMx><<<grid, block, 0, stream>>>(a);
-      else rms_norm_kernel<32, 4, kMx><<<grid, block, 0, stream>>>(a);
-      break;
-    case 128: rms_norm_kernel<128, 4, kMx><<<grid, block, 0, stream>>>(a); break;
-    case 256: rms_norm_kernel<256, 4, kMx><<<grid, block, 0, stream>>>(a); break;
-    default: rms_norm_kernel<512, 4, kMx><<<grid, block, 0, stream>>>(a); break;
-  }
+  if (threads > 32) rms_norm_kernel<false, kVectors, kMx><<<grid, block, 0, stream>>>(a);
+  else if (vec == 1) rms_norm_kernel<true, 1, kMx><<<grid, block, 0, stream>>>(a);
+  else if (vec == 2) rms_norm_kernel<true, 2, kMx><<<grid, block, 0, stream>>>(a);
+  else rms_norm_kernel<true, 4, kMx><<<grid, block, 0, stream>>>(a);
 }
 
 cudaError_t rms_norm(const fuse_b200_rms_norm_params& p, cudaStream_t stream) {
@@ -523,12 +523,8 @@ cudaError_t rms_norm_backward(const fuse_b200_rms_norm_backward_params& p, cudaS
   if (grid > 0) {
     const int vec = (p.hidden + threads * 8 - 1) / (threads * 8);
     const uint32_t shared = uint32_t(2 * 3 * 2 * p.hidden);
-    if (threads == 128) {
-      status = host::launch_kernel(rms_norm_backward_kernel<128>, int(grid), 128, shared, false, stream, a);
-    } else if (threads == 256) {
-      status = host::launch_kernel(rms_norm_backward_kernel<256>, int(grid), 256, shared, false, stream, a);
-    } else if (threads == 512) {
-      status = host::launch_kernel(rms_norm_backward_kernel<512>, int(grid), 512, shared, false, stream, a);
+    if (threads > 32) {
+      status = host::launch_kernel(rms_norm_backward_kernel, int(grid), threads, shared, false, stream, a);
     } else {
       if (vec == 1) rms_norm_backward_warp_kernel<1><<<grid, 128, 0, stream>>>(a);
       else rms_norm_backward_warp_kernel<2><<<grid, 128, 0, stream>>>(a);
