@@ -14,11 +14,14 @@
 // Roles (12 warps): warp 0 loads (TMA: both Q tiles, then K and V tiles through two rings), warps 1 and 3 issue the
 // UMMAs of one tile each, warp 2 allocates TMEM, warps 4-7 and 8-11 are one softmax group per tile, one thread per row.
 // TMEM (512 columns): S of either tile (128 FP32 columns each; P overwrites the first 64 of its own S as
-// packed BF16 and is the A operand of P V straight from there) and O of either tile.
+// packed BF16 and is the A operand of P V straight from there) and O of either tile.  With heads of 64 O takes half as
+// much, and P has columns of its own.
 //
 // The UMMAs of a tile are issued in the order P V, S of the next keys: while one tile's softmax runs, the tensor cores
 // work for the other.  They execute in issue order, so S may overwrite the P that the UMMA before it reads, and "S of
 // the next keys is complete" implies "O holds all keys before", which is what a softmax group needs to rescale O in place.
+// With heads of 64 S of the next keys is issued first, as soon as the softmax group has read this one's, and P V's completion
+// is waited for by itself.
 //
 // Few queries (one tile of them) against many keys: the keys are split over blocks, and within a block both tiles hold
 // the same queries and take every other key tile, so that one's softmax overlaps the other's products and the loads keep
@@ -262,8 +265,10 @@ struct ForwardLayout {
   static constexpr uint32_t kK = 2 * kTileBytes;
   static constexpr uint32_t kV = kK + kStages * kTileBytes;
   static constexpr uint32_t kBarriers = kV + kStages * kTileBytes;
-  // q_full[2], s_full[2], p_ready[2], drain[2], o_full, then k_full, k_empty, v_full, v_empty [kStages]
-  static constexpr uint32_t kNumBarriers = 9 + 4 * kStages;
+  // q_full[2], s_full[2], p_ready[2], drain[2], s_read[2], o_done[2], o_full, then k_full, k_empty, v_full, v_empty [kStages]
+  static constexpr uint32_t kNumBarriers = 13 + 4 * kStages;
+  // Heads of 64 leave TMEM for P beside S: S of the next keys is then issued as soon as this one's is in registers.
+  static constexpr bool kOwnP = kDim == 64;
   static constexpr uint32_t kSlot = kBarriers + kNumBarriers * 8;
   static constexpr uint32_t kDynamicBytes = kSlot + 16;
   static_assert(kDynamicBytes <= 227 * 1024, "shared memory budget");
@@ -309,11 +314,13 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   auto s_full = [&](int t) { return bars + 8u * (2 + t); };
   auto p_ready = [&](int t) { return bars + 8u * (4 + t); };
   auto drain = [&](int t) { return bars + 8u * (6 + t); };
-  const uint32_t o_full = bars + 8u * 8;
-  auto k_full = [&](int s) { return bars + 8u * (9 + s); };
-  auto k_empty = [&](int s) { return bars + 8u * (9 + kStages + s); };
-  auto v_full = [&](int s) { return bars + 8u * (9 + 2 * kStages + s); };
-  auto v_empty = [&](int s) { return bars + 8u * (9 + 3 * kStages + s); };
+  auto s_read = [&](int t) { return bars + 8u * (8 + t); };
+  auto o_done = [&](int t) { return bars + 8u * (10 + t); };
+  const uint32_t o_full = bars + 8u * 12;
+  auto k_full = [&](int s) { return bars + 8u * (13 + s); };
+  auto k_empty = [&](int s) { return bars + 8u * (13 + kStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (13 + 2 * kStages + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (13 + 3 * kStages + s); };
   auto k_tile = [&](int s) { return base + Layout::kK + s * Layout::kTileBytes; };
   auto v_tile = [&](int s) { return base + Layout::kV + s * Layout::kTileBytes; };
 
@@ -326,6 +333,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       ptx::mbar_init(s_full(t), 1);
       ptx::mbar_init(drain(t), 1);
       ptx::mbar_init(p_ready(t), 4);  // one arrival per warp of the softmax group
+      ptx::mbar_init(s_read(t), 4);
+      ptx::mbar_init(o_done(t), 1);
     }
     ptx::mbar_init(o_full, 2);  // from here on 2: a commit of either issuing warp
     for (int s = 0; s < kStages; ++s) {
@@ -345,7 +354,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   ptx::tc_fence_after();
   constexpr uint32_t tmem = 0;  // all 512 columns are this block's
   auto s_tmem = [&](int t) { return tmem + uint32_t(t) * 128u; };
-  auto o_tmem = [&](int t) { return tmem + 256u + uint32_t(t) * 128u; };
+  auto o_tmem = [&](int t) { return tmem + 256u + uint32_t(t) * kDim; };
+  auto p_tmem = [&](int t) { return Layout::kOwnP ? tmem + 384u + uint32_t(t) * 64u : s_tmem(t); };
 
   bool unwound = false;
   // 168 registers a thread at launch, 64,512 in all: 88 for the first four warps and 208 for the eight softmax warps
@@ -389,19 +399,33 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       uint32_t p_phase = 0, has_o = 0;
       uint32_t s = 0, s_next = 0, v_phase = 0, k_phase = 0;  // stages of V of tile `it` and of K of tile it + 1
       bool now = false, next = seen(it0);
+      uint32_t read_phase = 0, issued = 0;
+      auto scores = [&]() __attribute__((always_inline)) {
+        mma_rows<kDim>(issue, s_tmem(t), q_tile, k_tile(s_next));
+        ptx::umma_commit_if(issue, s_full(t));
+      };
       for (int32_t it = it0 - 1; ok && it < it1; ++it) {
         if (it + 1 < it1 && !(ok = warp_wait(k_full(s_next), k_phase, a.wait, kSiteSmemFull))) break;
+        if constexpr (Layout::kOwnP) {
+          if (next) {  // behind P V of the keys before, ahead of P V of these
+            if (issued && !(ok = warp_wait(s_read(t), read_phase, a.wait, kSiteTmemEmpty))) break;
+            read_phase ^= issued;
+            issued = 1;
+            ptx::tc_fence_after();
+            scores();
+          }
+        }
         if (it >= it0 && !(ok = warp_wait(v_full(s), v_phase, a.wait, kSiteSmemFull))) break;
         if (now) {
           if (!(ok = warp_wait(p_ready(t), p_phase, a.wait, kSiteTmemEmpty))) break;
           ptx::tc_fence_after();
-          mma_weights<kDim>(issue, o_tmem(t), Columns{s_tmem(t)}, v_tile(s), has_o);
+          mma_weights<kDim>(issue, o_tmem(t), Columns{p_tmem(t)}, v_tile(s), has_o);
+          if constexpr (Layout::kOwnP) ptx::umma_commit_if(issue, o_done(t));
           has_o = 1;
           p_phase ^= 1u;
         }
-        if (next) {
-          mma_rows<kDim>(issue, s_tmem(t), q_tile, k_tile(s_next));
-          ptx::umma_commit_if(issue, s_full(t));
+        if constexpr (!Layout::kOwnP) {
+          if (next) scores();
         }
         if (it >= it0) ptx::umma_commit_if(issue, v_empty(s));
         if (it + 1 < it1) ptx::umma_commit_if(issue, k_empty(s_next));
@@ -442,6 +466,11 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
       for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(s_at + i * 32, s[i]);
       ptx::tmem_wait_ld();
+      if constexpr (Layout::kOwnP) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(s_read(t));
+      }
       if (needs_mask(a, seq, my_first, my_last, k0, kTile)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -460,13 +489,17 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       const float largest = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
       if (largest != largest) l = largest;  // a score that is no number: so is the row
+      if constexpr (Layout::kOwnP) {  // P V of the keys before: O is complete, and P may be written again
+        if (begun && !(ok = warp_wait(o_done(t), phase, a.wait, kSiteTmemFull))) break;
+        ptx::tc_fence_after();
+      }
       if (__any_sync(0xffffffffu, largest > m + 8.0f)) {
         const float to = fmaxf(m, largest);
         const float factor = m == -INFINITY ? 0.0f : exp2_approx(m - to);
         l *= factor;
         m = to;
         if (begun) {
-          // O of the keys before is complete: S of this tile was issued behind it
+          // O of the keys before is complete: S of this tile was issued behind it (or it has been waited for above)
 #pragma unroll
           for (int c = 0; c < kDim; c += 32) {
             uint32_t o[32];
@@ -500,7 +533,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           sum[i] = c ? add2(sum[i], pair(x, y)) : pair(x, y);
           p[c] = pack_bf16(x, y);
         }
-        ptx::tmem_st_32x32b_x16(s_at + i * 16, p);
+        ptx::tmem_st_32x32b_x16(p_tmem(t) + lanes + i * 16, p);
       }
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
