@@ -247,7 +247,7 @@ class _Rotary(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, = ctx.saved_tensors
-        dq, dk = (None if g is None else _grad(g) for g in (dq, dk))
+        dq, dk = (_grad(g) if g is not None and needed else None for g, needed in zip((dq, dk), ctx.needs_input_grad))
         if dq is None and dk is None:
             return (None,) * 7
         oq, ok = (None if g is None else torch.empty(g.shape, dtype=BF16, device=g.device) for g in (dq, dk))
@@ -396,9 +396,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
 
     The rows are `batch` sequences of q_len queries and kv_len keys (default: all rows, evenly), one behind the other.
     Shorter ones have their lengths in q_lengths / kv_lengths, others their first rows in q_starts / kv_starts
-    (int32 [batch] on the device; q_len and kv_len are then the longest).  Queries are the last q_length
-    positions of their sequence.  Sequences may share keys (equal kv_starts) only without gradients.  With `causal`, `window` limits a query to the last `window` keys up to its own and the
-    first `sinks` of the sequence.  Rows of no sequence are zeros in the result (with `out`: as they were).
+    (int32 [batch] on the device; q_len and kv_len are then the longest).  Sequences may share keys (equal
+    kv_starts) only without gradients.  Queries are the last q_length positions of their sequence.  With `causal`,
+    `window` limits a query to the last `window` keys up to its own and the first `sinks` of the sequence.  Rows of
+    no sequence are zeros in the result (with `out`: as they were).
     `out`: a tensor to write to, such as UlyssesProjections.attention_buffer() -- without gradients only, since a
     later call would overwrite what the backward needs.  `return_lse`: also FP32 [q_heads, rows], no gradient."""
     _rows(q, "q")

@@ -274,7 +274,8 @@ cudaError_t rotary(const fuse_b200_rotary_params& p, cudaStream_t stream) {
     // rows per block: one batch of every thread, while the angles stay within 24 KiB
     const int64_t slots = int64_t(p.q_heads + p.kv_heads) * (d / 16);
     int64_t tokens = slots < kBlock ? kBatch * (kBlock / slots) : kBatch;
-    if (tokens * (n / 2) > 3072) tokens = 3072 / (n / 2);
+    constexpr int64_t kTurns = 24 * 1024 / sizeof(float2);
+    if (tokens * (n / 2) > kTurns) tokens = kTurns / (n / 2);
     const int64_t chunks = (p.rows + tokens - 1) / tokens, resident = int64_t(info.sm_count) * 8;
     const unsigned grid = unsigned(chunks < resident ? chunks : resident);
     const size_t shared = size_t(tokens) * (n / 2) * sizeof(float2);

@@ -652,7 +652,7 @@ FUSE_API int fuse_b200_launch_rotary(const fuse_b200_rotary_params* params, fuse
 
 /* Attention of q_len queries per sequence over kv_len keys, between the two all-to-alls: q
  * [q_rows, q_heads * head_dim], k and v [kv_rows, kv_heads * head_dim], output like q -- the [rows, heads * d]
- * tensor the output projection reads.  head_dim 64 or 128; q_heads a multiple of kv_heads (query head h reads
+ * tensor the output projection reads.  head_dim 64 or 128 (others: not supported); q_heads a multiple of kv_heads (query head h reads
  * KV head h / (q_heads / kv_heads)).  Strides multiples of 8, pointers 16-byte aligned.
  *
  * Sequence b has q_lengths[b] <= q_len queries from row q_starts[b] on and kv_lengths[b] <= kv_len keys from row
