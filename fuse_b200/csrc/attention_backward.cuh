@@ -13,7 +13,9 @@
 // columns, one thread per row and half.  The first kernel's dQ has an issuing warp of its own (192 -> 187 us at
 // 8192 x 8 heads); the second kernel's four products keep one order, dV, S of the next tile, dK, dP of the next (two
 // warps: 245 -> 319 us).  P and dS are rounded to BF16 for their products, as every operand of
-// the tensor cores is; they are made from FP32 scores and dP and accumulated in FP32.
+// the tensor cores is; they are made from FP32 scores and dP and accumulated in FP32.  D comes from the rounded O:
+// adding back what O's rounding took off moved dQ's error from 0.03399 to 0.03384 and dK's not at all (norms; 512 x 2048,
+// 4 / 1 heads of 64), so it is not kept.
 #pragma once
 
 #include "attention.cuh"
