@@ -202,6 +202,14 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const W
   }
 }
 
+// A warp arrives with one lane.  tcgen05.ld, .st, .wait and the named barriers are .sync.aligned: behind every branch that
+// lanes take apart (this one, a row's store, zeroed rows) the warp is brought together before it comes to the next of them.
+__device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
+  __syncwarp();
+  if (lane == 0) ptx::mbar_arrive(bar);
+  __syncwarp();
+}
+
 // A [128 x kDim] BF16 tile in shared memory: kDim / 64 blocks of 128 rows x 128 bytes, 128-byte swizzle.
 template <int kDim>
 struct TileShape {
@@ -227,6 +235,7 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int32_t row, int32_t va
         ptx::st_shared_v4(tile + b * TileShape<kDim>::kBlockBytes + uint32_t(row) * 128u + i * 16u, make_uint4(0u, 0u, 0u, 0u));
   }
   ptx::fence_proxy_async_shared();
+  __syncwarp();
 }
 
 // D[128 x kColumns] = A B^T over kDim: both operands K-major tiles, of B the kColumns rows from `b_tile` on.
@@ -345,6 +354,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     ptx::fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 2) {
     ptx::tmem_alloc(base + Layout::kSlot, 512);
     ptx::tmem_relinquish();
@@ -468,8 +478,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       ptx::tmem_wait_ld();
       if constexpr (Layout::kOwnP) {
         ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(s_read(t));
+        warp_arrive(s_read(t), lane);
       }
       if (needs_mask(a, seq, my_first, my_last, k0, kTile)) {
 #pragma unroll
@@ -488,7 +497,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         top[i] = max3(top[i], as_float(s[i][31]), as_float(s[i][31]));
       }
       const float largest = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
-      if (largest != largest) l = largest;  // a score that is no number: so is the row
+      l = largest != largest ? largest : l;  // a score that is no number: so is the row
       if constexpr (Layout::kOwnP) {  // P V of the keys before: O is complete, and P may be written again
         if (begun && !(ok = warp_wait(o_done(t), phase, a.wait, kSiteTmemFull))) break;
         ptx::tc_fence_after();
@@ -537,8 +546,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(p_ready(t));
+      warp_arrive(p_ready(t), lane);
       float l0, l1;
       unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
       l += l0 + l1;
@@ -562,6 +570,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
         for (int c = 0; c < kDim; c += 32) {
           uint32_t o[32];
+          __syncwarp();
           ptx::tmem_ld_32x32b_x32(o_at + c, o);
           ptx::tmem_wait_ld();
 #pragma unroll
@@ -589,6 +598,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint64_t start = ptx::globaltimer();
     while (ptx::globaltimer() - start < 200000ull) __nanosleep(1000);
   }
+  __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
   if (warp == 2) {

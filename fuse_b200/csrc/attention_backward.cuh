@@ -141,6 +141,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     }
     ptx::fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 2) {
     ptx::tmem_alloc(base + Layout::kSlot, 512);
     ptx::tmem_relinquish();
@@ -240,6 +241,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     }
     float* parts = reinterpret_cast<float*>(smem_raw + Layout::kDelta);
     parts[half * kTile + row] = part;
+    __syncwarp();
     ptx::named_bar_sync(1, kElementwiseThreads);
     const float delta = parts[row] + parts[kTile + row];
     const int64_t stat = int64_t(head) * a.q_rows + q_row;
@@ -249,6 +251,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       lse = ba.lse[stat] * kLog2e;
       if (lse == -INFINITY) lse = INFINITY;
     }
+    __syncwarp();
     const int32_t pos = token + seq.off;
     const int32_t hi = a.causal ? min(pos, seq.kl - 1) : seq.kl - 1;
     const int32_t lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
@@ -265,8 +268,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       ptx::tmem_ld_32x32b_x32(s_tmem + lanes + columns + 32, s[1]);
       ptx::tmem_wait_ld();
       ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(s_read);
+      warp_arrive(s_read, lane);
       const bool masked = needs_mask(a, seq, first, last, k0, kTile);
       if (masked) {
 #pragma unroll
@@ -305,8 +307,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       }
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ds_ready(slot));
+      warp_arrive(ds_ready(slot), lane);
     }
     if (ok) {
       if (tiles.count > 0) ok = warp_wait(dq_full, 0, a.wait, kSiteTmemFull);
@@ -316,6 +317,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         for (int c = 0; c < kDim / 2; c += 32) {
           uint32_t v[32];
           const int32_t column = half * (kDim / 2) + c;
+          __syncwarp();
           ptx::tmem_ld_32x32b_x32(dq_tmem + lanes + uint32_t(column), v);
           ptx::tmem_wait_ld();
           if (tiles.count == 0) {
@@ -332,6 +334,7 @@ attention_query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const uint64_t start = ptx::globaltimer();
     while (ptx::globaltimer() - start < 200000ull) __nanosleep(1000);
   }
+  __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
   if (warp == 2) {
@@ -441,6 +444,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     }
     ptx::fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 2) {
     ptx::tmem_alloc(base + Layout::kSlot, 512);
     ptx::tmem_relinquish();
@@ -529,8 +533,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         mine[i * 32 + lane] = lse[i];
         mine[kTile + i * 32 + lane] = delta[i];
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(stat_full(j & 1));
+      warp_arrive(stat_full(j & 1), lane);
     }
     unwound = !ok;
   } else if (warp >= 4) {
@@ -598,8 +601,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(p_ready);
+      warp_arrive(p_ready, lane);
       if (!(ok = warp_wait(dp_full, j & 1, a.wait, kSiteTmemFull))) break;
       ptx::tc_fence_after();
 #pragma unroll
@@ -634,6 +636,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         ptx::mbar_arrive(stat_empty(j & 1));
         ptx::mbar_arrive(ds_ready);
       }
+      __syncwarp();
     }
     if (ok) {
       if (total > 0) ok = warp_wait(grads_full, 0, a.wait, kSiteTmemFull);
@@ -647,6 +650,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           for (int c = 0; c < kDim / 2; c += 32) {
             uint32_t v[32];
             const int32_t column = half * (kDim / 2) + c;
+            __syncwarp();
             ptx::tmem_ld_32x32b_x32((which ? dk_tmem : dv_tmem) + lanes + uint32_t(column), v);
             ptx::tmem_wait_ld();
             if (total == 0) {
@@ -672,6 +676,7 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint64_t start = ptx::globaltimer();
     while (ptx::globaltimer() - start < 200000ull) __nanosleep(1000);
   }
+  __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
   if (warp == 2) {
