@@ -577,8 +577,9 @@ attention_key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
       }
       if (masked) {
-        // the columns of tokens [from, to): those in [low, high)
-        const int32_t low = (max(from, t0) - t0) << a.pack_shift, high = (min(to, t0 + tile_tokens) - t0) * a.pack;
+        // the columns of tokens [from, to): those in [low, high).  Tokens are brought into the tile before they are multiplied by its
+        // heads: in a tile with sinks `to` can lie a whole context away, and that times 128 heads is past 31 bits
+        const int32_t low = min(max(from - t0, 0), tile_tokens) << a.pack_shift, high = min(max(to - t0, 0), tile_tokens) << a.pack_shift;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int32_t at = int32_t(columns) + i * 32;
