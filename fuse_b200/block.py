@@ -71,6 +71,14 @@ class _On:
             torch.cuda.set_device(self.back)
 
 
+def _written(*tensors) -> None:
+    """What a kernel has written through its pointer counts as modified in place: autograd then refuses a backward that had
+    saved it, as it does for torch's own in-place operations."""
+    for t in tensors:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -292,6 +300,7 @@ def rotary_(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, hea
     if _wants_grad(q, k):
         raise RuntimeError("rotary_ writes its arguments and has no gradient: use rotary")
     _rotary_launch(q, k, q, k, record, head_dim, seq_len, start, positions, 0)
+    _written(q, k)
     return q, k
 
 
@@ -424,5 +433,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
             raise RuntimeError("out= would be overwritten before the backward has read it: leave it out, or use torch.no_grad()")
         out, lse = _Attention.apply(q, k, v, shape, "whole" if return_lse else "own")
     else:
-        out, lse = _attention_forward(q, k, v, shape, out, "whole" if return_lse else None)
+        given = out
+        out, lse = _attention_forward(q, k, v, shape, given, "whole" if return_lse else None)
+        _written(given)
     return (out, lse) if return_lse else out

@@ -1,0 +1,51 @@
+"""What the block operators (fuse_b200/block.py) owe to autograd and to their arguments: writes that autograd sees."""
+import pytest
+import torch
+
+from fuse_b200 import block
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16 = torch.bfloat16
+SPEC = block.Rotary(64)
+
+
+def randn(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(BF16)
+
+
+# ---- writes in place are seen
+def test_a_tensor_turned_in_place_is_not_taken_for_the_saved_one():
+    q, k, v = (randn(40, 64, seed=i).requires_grad_() for i in range(3))
+    kept = k * 1  # no leaf
+    o = block.attention(q, kept, v, head_dim=64)
+    with torch.no_grad():
+        block.rotary_(None, kept, SPEC, head_dim=64)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+
+
+def test_an_output_written_over_a_saved_tensor_is_not_taken_for_it():
+    q, k, v = (randn(40, 64, seed=i).requires_grad_() for i in range(3))
+    kept = q * 1
+    o = block.attention(kept, k, v, head_dim=64)
+    with torch.no_grad():
+        block.attention(k, k, v, head_dim=64, out=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+
+
+def test_versions_count_writes():
+    q, k = randn(8, 128), randn(8, 64)
+    before = q._version, k._version
+    block.rotary(q, k, SPEC, head_dim=64)
+    assert (q._version, k._version) == before
+    block.rotary_(q, k, SPEC, head_dim=64)
+    assert q._version > before[0] and k._version > before[1]
+    out = torch.empty_like(k)
+    before = out._version
+    block.attention(k, k, k, head_dim=64, out=out)
+    assert out._version > before
+    with torch.inference_mode():  # inference tensors have no versions
+        block.rotary_(q.clone(), None, SPEC, head_dim=64)
+        block.attention(k, k, k, head_dim=64, out=torch.empty_like(k))
