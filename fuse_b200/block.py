@@ -7,13 +7,14 @@
 Tensors are BF16 [rows, width] on one CUDA device, rows `width` apart or more (views of wider tensors
 do, with row strides of a multiple of 8 elements); a tensor that an operator cannot take is refused, never copied.
 Work runs on the tensors' device and on its current stream.  Gradients come through torch.autograd
-where an argument requires them.  The C entry points underneath are in include/fuse_b200.h."""
+where an argument requires them; forward mode is refused.  The C entry points underneath are in include/fuse_b200.h."""
 from __future__ import annotations
 
 import ctypes as C
 import dataclasses
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -80,6 +81,10 @@ def _written(*tensors) -> None:
 
 
 def _wants_grad(*tensors) -> bool:
+    # a tensor in forward mode need not require a gradient; its tangent would be dropped, that is, taken for zero
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the block operators have no forward-mode derivative (torch.autograd.forward_ad, torch.func.jvp)")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

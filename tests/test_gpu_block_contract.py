@@ -1,6 +1,8 @@
-"""What the block operators (fuse_b200/block.py) owe to autograd and to their arguments: writes that autograd sees."""
+"""What the block operators (fuse_b200/block.py) owe to autograd and to their arguments: writes that autograd sees, forward-mode
+tangents."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from fuse_b200 import block
 
@@ -49,3 +51,21 @@ def test_versions_count_writes():
     with torch.inference_mode():  # inference tensors have no versions
         block.rotary_(q.clone(), None, SPEC, head_dim=64)
         block.attention(k, k, k, head_dim=64, out=torch.empty_like(k))
+
+
+# ---- forward mode has no derivative here: refused, not dropped
+def test_forward_mode_is_refused():
+    x, gamma, q, k, v = randn(8, 256), randn(256), randn(8, 64), randn(8, 64), randn(8, 64)
+    calls = [(x, lambda t: block.rms_norm(t, gamma)), (gamma, lambda t: block.rms_norm(x, t)), (x, lambda t: block.rms_norm(x, gamma, t)),
+             (x, lambda t: block.rms_norm(t, gamma, mxfp8=True)), (x, lambda t: block.rms_norm_mxfp8(t, gamma)),
+             (q, lambda t: block.rotary(t, k, SPEC, head_dim=64)), (k, lambda t: block.rotary(q, t, SPEC, head_dim=64)),
+             (q, lambda t: block.rotary_(t, None, SPEC, head_dim=64)),
+             (q, lambda t: block.attention(t, k, v, head_dim=64)), (k, lambda t: block.attention(q, t, v, head_dim=64)),
+             (v, lambda t: block.attention(q, k, t, head_dim=64))]
+    for primal, call in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward"):
+                call(forward_ad.make_dual(primal.clone(), torch.ones_like(primal)))
+            call(primal.clone())  # without a tangent it runs
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (primal,), (torch.ones_like(primal),))
