@@ -433,6 +433,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
              head_dim ** -0.5 if scale is None else scale, q_starts, q_lengths, kv_starts, kv_lengths)
     if out is not None:
         _rows(out, "out", q.shape[1], q.shape[0], q.device)
+        if _wants_grad(out):
+            raise RuntimeError("out= is written in place and must not require a gradient: pass out.detach(), or use torch.no_grad()")
     if _wants_grad(q, k, v):
         if out is not None:
             raise RuntimeError("out= would be overwritten before the backward has read it: leave it out, or use torch.no_grad()")

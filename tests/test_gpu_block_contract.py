@@ -69,3 +69,16 @@ def test_forward_mode_is_refused():
             call(primal.clone())  # without a tangent it runs
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (primal,), (torch.ones_like(primal),))
+
+
+def test_an_output_of_its_own_derivative_is_refused():
+    q, out = randn(8, 64), randn(8, 64, seed=1)
+    keep = out.clone()
+    with pytest.raises(RuntimeError, match="gradient"):
+        block.attention(q, q, q, head_dim=64, out=out.requires_grad_())
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward"):
+        block.attention(q, q, q, head_dim=64, out=forward_ad.make_dual(out.detach(), torch.ones_like(out)))
+    assert torch.equal(out, keep)
+    with torch.no_grad():
+        block.attention(q, q, q, head_dim=64, out=out)
+    assert torch.equal(out, block.attention(q, q, q, head_dim=64))
