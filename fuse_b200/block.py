@@ -47,6 +47,26 @@ def _grad(g: torch.Tensor) -> torch.Tensor:
     return g.clone(memory_format=torch.contiguous_format)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the rows of two tensors reach a common element (columns of one wider tensor, side by side, do not)."""
+    if not a.numel() or not b.numel():
+        return False
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    gap, (n, width), (m, other) = (b.data_ptr() - a.data_ptr()) // a.element_size(), a.shape, b.shape
+    if gap >= (n - 1) * a.stride(0) + width:
+        return False
+    pitch = a.stride(0)
+    if n == 1 or pitch < width:
+        return True
+    # b's rows against a's: with one pitch all of them start in the same column, and the first decides
+    for at in range(gap, gap + 1 if m == 1 or b.stride(0) == pitch else gap + m * b.stride(0), max(b.stride(0), 1)):
+        row, column = divmod(at, pitch)
+        if (row < n and column < width) or (row + 1 < n and column + other > pitch):
+            return True
+    return False
+
+
 try:  # the stream's handle without the Stream object around it: 0.1 us instead of 1.4
     from torch._C import _cuda_getCurrentRawStream as _raw_stream
 except ImportError:
@@ -300,10 +320,12 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head
 
 def rotary_(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head_dim: int, seq_len: int | None = None,
             start: int = 0, positions: torch.Tensor | None = None):
-    """The same in place (no gradient)."""
+    """The same in place (no gradient); q and k must not share memory."""
     record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, positions)
     if _wants_grad(q, k):
         raise RuntimeError("rotary_ writes its arguments and has no gradient: use rotary")
+    if q is not None and k is not None and _overlap(q, k):
+        raise ValueError("q and k share memory: each would be turned while the other is read")
     _rotary_launch(q, k, q, k, record, head_dim, seq_len, start, positions, 0)
     _written(q, k)
     return q, k
@@ -415,7 +437,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
     `window` limits a query to the last `window` keys up to its own and the first `sinks` of the sequence.  Rows of
     no sequence are zeros in the result (with `out`: as they were).
     `out`: a tensor to write to, such as UlyssesProjections.attention_buffer() -- without gradients only, since a
-    later call would overwrite what the backward needs.  `return_lse`: also FP32 [q_heads, rows], no gradient."""
+    later call would overwrite what the backward needs; it must not share memory with q, k or v.  `return_lse`: also FP32 [q_heads, rows], no gradient."""
     _rows(q, "q")
     _rows(k, "k", device=q.device)
     _rows(v, "v", k.shape[1], k.shape[0], q.device)
@@ -435,6 +457,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
         _rows(out, "out", q.shape[1], q.shape[0], q.device)
         if _wants_grad(out):
             raise RuntimeError("out= is written in place and must not require a gradient: pass out.detach(), or use torch.no_grad()")
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            if _overlap(out, t):
+                raise ValueError(f"out and {name} share memory")
     if _wants_grad(q, k, v):
         if out is not None:
             raise RuntimeError("out= would be overwritten before the backward has read it: leave it out, or use torch.no_grad()")

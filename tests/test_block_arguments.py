@@ -1,0 +1,28 @@
+"""Host arithmetic behind the block operators' refusals (fuse_b200/block.py)."""
+import random
+
+import torch
+
+from fuse_b200 import block
+
+
+def test_overlap_of_row_views_against_enumeration():
+    base = torch.arange(400, dtype=torch.int32)
+    rng = random.Random(3)
+    seen = {True: 0, False: 0}
+    for _ in range(6000):
+        views = []
+        pitch = rng.choice((7, 12, 20))
+        for _ in range(2):
+            if rng.random() < 0.2:
+                pitch = rng.choice((7, 12, 20))
+            rows, width = rng.randint(1, 5), rng.randint(1, pitch)
+            views.append(base.as_strided((rows, width), (pitch, 1), rng.randint(0, 200)))
+        a, b = views
+        want = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert block._overlap(a, b) == block._overlap(b, a) == want, (a, b)
+        seen[want] += 1
+    assert min(seen.values()) > 1000
+    assert not block._overlap(base[:0].view(0, 4), base.view(100, 4))
+    half = base.view(torch.bfloat16).view(100, 8)
+    assert block._overlap(half[:, :4], half[:, 3:]) and not block._overlap(half[:, :4], half[:, 4:])

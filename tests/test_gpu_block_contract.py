@@ -1,5 +1,5 @@
 """What the block operators (fuse_b200/block.py) owe to autograd and to their arguments: writes that autograd sees, forward-mode
-tangents."""
+tangents, memory that two arguments share."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -82,3 +82,31 @@ def test_an_output_of_its_own_derivative_is_refused():
     with torch.no_grad():
         block.attention(q, q, q, head_dim=64, out=out)
     assert torch.equal(out, block.attention(q, q, q, head_dim=64))
+
+
+# ---- arguments that share memory
+def test_rotary_in_place_refuses_shared_memory():
+    wide = randn(20, 512)
+    for q, k in ((wide, wide), (wide[:, :128], wide[:, 64:192]), (wide[:10], wide[:10]), (wide[:, :128], wide[:, :64]),
+                 (wide[0:1, :128], wide[0:1, 64:192])):
+        with pytest.raises(ValueError, match="share memory"):
+            block.rotary_(q, k, SPEC, head_dim=64)
+    keep = wide.clone()
+    block.rotary_(wide[:, :128], wide[:, 128:192], SPEC, head_dim=64)  # side by side
+    block.rotary_(wide[:10, 192:256], wide[10:, 192:256], SPEC, head_dim=64)  # one above the other
+    assert torch.equal(wide[:, 256:], keep[:, 256:])
+    turned, _ = block.rotary(keep[:, :128], None, SPEC, head_dim=64)
+    assert torch.equal(wide[:, :128], turned)
+    same, again = block.rotary(keep, keep, SPEC, head_dim=64)  # read twice is fine
+    assert torch.equal(same, again)
+
+
+def test_attention_refuses_an_output_over_an_input():
+    wide = randn(64, 512)
+    q, k, v = wide[:, :128], wide[:, 128:192], wide[:, 192:256]
+    for out in (q, wide[:, 64:192], wide[:, 192:320]):
+        with pytest.raises(ValueError, match="share memory"):
+            block.attention(q, k, v, head_dim=64, out=out)
+    want = block.attention(q, k, v, head_dim=64)
+    block.attention(q, k, v, head_dim=64, out=wide[:, 256:384])  # beside them
+    assert torch.equal(wide[:, 256:384], want)
