@@ -45,8 +45,9 @@ int32_t plan_splits(const fuse_b200_attention_params& p, int sm_count) {
   const int64_t blocks = query_blocks(p);
   int64_t keys = p.kv_len;
   const int64_t seen = int64_t(p.window) + p.q_len;
-  if (p.window > 0 && seen < keys) keys = seen + (p.sinks < keys - seen ? p.sinks : keys - seen);
-  const int64_t tiles = (keys + attn::kTile - 1) / attn::kTile + (p.window > 0 ? 1 : 0);
+  const bool limited = p.window > 0 && p.window < p.kv_len;  // as the kernels take it: a longer window is none
+  if (limited && seen < keys) keys = seen + (p.sinks < keys - seen ? p.sinks : keys - seen);
+  const int64_t tiles = (keys + attn::kTile - 1) / attn::kTile + (limited ? 1 : 0);
   if (blocks == 0 || blocks >= sm_count || tiles < 4) return 1;
   constexpr double kFixed = 5.0, kJoin = 2.0;
   double best = double(tiles) + kFixed;

@@ -1,4 +1,4 @@
-"""Attention whose positions lie far along a long cache: gradients of a window and sinks past 16 million keys, where a position
+"""Attention at the ends of its ranges.  Positions far along a long cache: gradients of a window and sinks past 16 million keys, where a position
 times the heads of a tile no longer fits 31 bits (csrc/attention_backward.cuh).  What lies between the sinks and the window is
 seen by nobody, so the same tensors without it give the same results; tolerances: attention_reference.py."""
 import pytest
@@ -37,3 +37,17 @@ def test_sinks_and_window_far_apart(window, sinks):
     assert not dk[sinks:kv_len - tail].any() and not dv[sinks:kv_len - tail].any()  # seen by nobody
     got = {"o": out.detach(), "dq": dq, **{n: torch.cat((t[:head], t[kv_len - tail:])) for n, t in (("dk", dk), ("dv", dv))}}
     check(got, want, ["o", "dq", "dk", "dv"])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 129, 300, 600])
+def test_a_window_that_limits_nothing_changes_nothing(n, d):
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v, do = (torch.randn(n, d, generator=gen, device=DEV).to(BF16) for _ in range(4))
+    results = []
+    for kw in (dict(), dict(window=n), dict(window=(1 << 31) - 1, sinks=(1 << 31) - 1), dict(window=n + 1, sinks=5), dict(sinks=7)):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = block.attention(*leaves, head_dim=d, **kw)
+        results.append((out.detach(), *torch.autograd.grad(out, leaves, do)))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
