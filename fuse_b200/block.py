@@ -26,6 +26,13 @@ def _check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} -> cudaError {rc}")
 
 
+def _within(bits: int, **numbers: int) -> None:
+    """Whole numbers that a record's signed field of `bits` holds (ctypes would cut off the rest without a word)."""
+    for name, value in numbers.items():
+        if not -(1 << (bits - 1)) <= value < 1 << (bits - 1):
+            raise ValueError(f"{name}: {value} does not fit {bits} bits")
+
+
 def _rows(t: torch.Tensor, name: str, width: int | None = None, rows: int | None = None, device=None) -> None:
     if (not isinstance(t, torch.Tensor) or t.dtype != BF16 or t.dim() != 2 or not t.is_cuda or
             (t.shape[1] != 1 and t.stride(1) != 1) or (width is not None and t.shape[1] != width) or
@@ -236,6 +243,8 @@ class Rotary:
     def record(self) -> N.RotarySpec:
         if self.scaling not in N.ROTARY_SCALINGS:
             raise ValueError(f"scaling: one of {sorted(N.ROTARY_SCALINGS)}, got {self.scaling!r}")
+        _within(32, rotary_dim=self.rotary_dim)
+        _within(64, original_context=self.original_context)
         return N.RotarySpec(self.theta, self.factor, self.low_freq_factor, self.high_freq_factor, self.beta_fast,
                             self.beta_slow, self.magnitude, self.original_context, self.rotary_dim,
                             N.ROTARY_SCALINGS[self.scaling], 1 if self.interleaved else 0)
@@ -289,7 +298,7 @@ class _Rotary(torch.autograd.Function):
         return oq, ok, None, None, None, None, None
 
 
-def _rotary_arguments(q, k, spec, head_dim, seq_len, positions):
+def _rotary_arguments(q, k, spec, head_dim, seq_len, start, positions):
     some = q if q is not None else k
     if some is None:
         raise ValueError("rotary needs q or k")
@@ -303,6 +312,7 @@ def _rotary_arguments(q, k, spec, head_dim, seq_len, positions):
         raise ValueError(f"positions: expected contiguous int32 or int64 ({some.shape[0]},) on {some.device}")
     if seq_len is None:
         seq_len = max(1, some.shape[0])
+    _within(64, seq_len=seq_len, start=start)
     return spec.record(), seq_len
 
 
@@ -310,7 +320,7 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head
            start: int = 0, positions: torch.Tensor | None = None):
     """Turned copies of q [rows, q_heads * head_dim] and k [rows, kv_heads * head_dim] (either may be None).  Row r is
     at position positions[r], or start + r % seq_len (seq_len: all rows, one sequence)."""
-    record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, positions)
+    record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, start, positions)
     if _wants_grad(q, k):
         return _Rotary.apply(q, k, record, head_dim, seq_len, start, positions)
     qo, ko = (None if t is None else torch.empty(t.shape, dtype=BF16, device=t.device) for t in (q, k))
@@ -321,7 +331,7 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head
 def rotary_(q: torch.Tensor | None, k: torch.Tensor | None, spec: Rotary, *, head_dim: int, seq_len: int | None = None,
             start: int = 0, positions: torch.Tensor | None = None):
     """The same in place (no gradient); q and k must not share memory."""
-    record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, positions)
+    record, seq_len = _rotary_arguments(q, k, spec, head_dim, seq_len, start, positions)
     if _wants_grad(q, k):
         raise RuntimeError("rotary_ writes its arguments and has no gradient: use rotary")
     if q is not None and k is not None and _overlap(q, k):
@@ -450,7 +460,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
             raise ValueError(f"{name}: expected contiguous int32 ({batch},) on {q.device}")
     if window < 0 or sinks < 0 or (window and not causal):
         raise ValueError("window and sinks are not negative, and a window goes with causal attention")
-    shape = (batch, q.shape[0] // batch if q_len is None else q_len, k.shape[0] // batch if kv_len is None else kv_len,
+    q_len, kv_len = q.shape[0] // batch if q_len is None else q_len, k.shape[0] // batch if kv_len is None else kv_len
+    _within(32, batch=batch, q_len=q_len, kv_len=kv_len, window=window, sinks=sinks)
+    shape = (batch, q_len, kv_len,
              q.shape[1] // head_dim, k.shape[1] // head_dim, head_dim, 1 if causal else 0, window, sinks,
              head_dim ** -0.5 if scale is None else scale, q_starts, q_lengths, kv_starts, kv_lengths)
     if out is not None:

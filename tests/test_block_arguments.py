@@ -1,6 +1,7 @@
 """Host arithmetic behind the block operators' refusals (fuse_b200/block.py)."""
 import random
 
+import pytest
 import torch
 
 from fuse_b200 import block
@@ -26,3 +27,15 @@ def test_overlap_of_row_views_against_enumeration():
     assert not block._overlap(base[:0].view(0, 4), base.view(100, 4))
     half = base.view(torch.bfloat16).view(100, 8)
     assert block._overlap(half[:, :4], half[:, 3:]) and not block._overlap(half[:, :4], half[:, 4:])
+
+
+def test_numbers_that_a_record_would_cut_off():
+    block._within(32, window=(1 << 31) - 1, sinks=-(1 << 31))
+    block._within(64, start=(1 << 63) - 1)
+    for bits, value in ((32, 1 << 31), (32, (1 << 32) + 5), (32, -(1 << 31) - 1), (64, 1 << 63), (64, (1 << 64) + 300)):
+        with pytest.raises(ValueError, match="window: "):
+            block._within(bits, window=value)
+    with pytest.raises(ValueError, match="rotary_dim"):
+        block.Rotary((1 << 32) + 64).record()
+    with pytest.raises(ValueError, match="original_context"):
+        block.Rotary(64, scaling="yarn", factor=2.0, original_context=(1 << 64) + 8192).frequencies()

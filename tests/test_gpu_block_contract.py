@@ -1,5 +1,5 @@
 """What the block operators (fuse_b200/block.py) owe to autograd and to their arguments: writes that autograd sees, forward-mode
-tangents, memory that two arguments share."""
+tangents, memory that two arguments share, numbers past 31 bits."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -110,3 +110,18 @@ def test_attention_refuses_an_output_over_an_input():
     want = block.attention(q, k, v, head_dim=64)
     block.attention(q, k, v, head_dim=64, out=wide[:, 256:384])  # beside them
     assert torch.equal(wide[:, 256:384], want)
+
+
+# ---- numbers past 31 bits
+def test_numbers_past_31_bits_are_refused():
+    q = randn(300, 64)
+    for kw in (dict(window=(1 << 32) + 5), dict(window=1 << 31), dict(window=5, sinks=1 << 32), dict(q_len=(1 << 32) + 300), dict(kv_len=(1 << 32) + 300)):
+        with pytest.raises(ValueError):
+            block.attention(q, q, q, head_dim=64, **kw)
+    whole = block.attention(q, q, q, head_dim=64)
+    assert torch.equal(block.attention(q, q, q, head_dim=64, window=(1 << 31) - 1, sinks=(1 << 31) - 1), whole)
+    with pytest.raises(ValueError):
+        block.rotary(q, None, block.Rotary((1 << 32) + 64), head_dim=64)
+    for kw in (dict(seq_len=(1 << 64) + 300), dict(start=1 << 63)):
+        with pytest.raises(ValueError):
+            block.rotary(q, None, SPEC, head_dim=64, **kw)
