@@ -1,5 +1,6 @@
 """What the block operators (fuse_b200/block.py) owe to autograd and to their arguments: writes that autograd sees, forward-mode
-tangents, memory that two arguments share, numbers past 31 bits."""
+tangents, memory that two arguments share, numbers past 31 bits, the gradient of
+the norm with two outputs."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -125,3 +126,18 @@ def test_numbers_past_31_bits_are_refused():
     for kw in (dict(seq_len=(1 << 64) + 300), dict(start=1 << 63)):
         with pytest.raises(ValueError):
             block.rotary(q, None, SPEC, head_dim=64, **kw)
+
+
+# ---- the norm that gives both forms at once has the gradient of the one that gives BF16
+@pytest.mark.parametrize("rows,hidden", [(1, 32), (130, 1024), (33, 5120), (5, 8224)])
+def test_gradient_beside_the_mxfp8_form(rows, hidden):
+    x, residual, gamma, dy, dh = randn(rows, hidden, seed=1), randn(rows, hidden, seed=2), randn(hidden, seed=3), randn(rows, hidden, seed=4), randn(rows, hidden, seed=5)
+    results = []
+    for mxfp8 in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, residual, gamma)]
+        y, h, *packed = block.rms_norm(leaves[0], leaves[2], leaves[1], mxfp8=mxfp8)
+        assert all(not t.requires_grad for t in packed)
+        results.append((y.detach(), h.detach(), *torch.autograd.grad((y, h), leaves, (dy, dh))))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    h2, data, scales = block.rms_norm_mxfp8(x, gamma, residual)
+    assert torch.equal(h2, results[1][1]) and torch.equal(data, packed[0]) and torch.equal(scales, packed[1])
