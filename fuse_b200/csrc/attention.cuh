@@ -238,11 +238,10 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int32_t row, int32_t va
   __syncwarp();
 }
 
-// D[128 x kColumns] = A B^T over kDim: both operands K-major tiles, of B the kColumns rows from `b_tile` on.
-// A converged warp.
-template <int kDim, int kColumns = kTile>
+// D[128 x 128] = A B^T over kDim: both operands K-major tiles.  A converged warp.
+template <int kDim>
 __device__ __forceinline__ void mma_rows(uint32_t issue, uint32_t d, uint32_t a_tile, uint32_t b_tile) {
-  constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kColumns, 0, 0);
+  constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kTile, 0, 0);
   const uint64_t a_desc = ptx::smem_desc_k_sw128(a_tile), b_desc = ptx::smem_desc_k_sw128(b_tile);
 #pragma unroll
   for (uint32_t k = 0; k < kDim / 16; ++k) {
@@ -250,14 +249,14 @@ __device__ __forceinline__ void mma_rows(uint32_t issue, uint32_t d, uint32_t a_
     ptx::umma_f16_if(issue, d, a_desc + at, b_desc + at, kIdesc, k != 0 ? 1u : 0u);
   }
 }
-// D[128 x kDim] (+)= A[128 x kRows] B: A in TMEM (K values 16 k .. 16 k + 15 at column a_column(k)), B the kRows rows of
-// a tile from `b_tile` on, which are the K axis.
-template <int kDim, int kRows = kTile, class Column>
+// D[128 x kDim] (+)= A[128 x 128] B: A in TMEM (K values 16 k .. 16 k + 15 at column a_column(k)), B a tile whose rows are
+// the K axis.
+template <int kDim, class Column>
 __device__ __forceinline__ void mma_weights(uint32_t issue, uint32_t d, Column a_column, uint32_t b_tile, bool accumulate) {
   constexpr uint32_t kIdesc = ptx::idesc_bf16_f32(kTile, kDim, 0, 1);
   const uint64_t b_desc = ptx::smem_desc_mn_sw128(b_tile, TileShape<kDim>::kBlockBytes);
 #pragma unroll
-  for (uint32_t k = 0; k < kRows / 16; ++k)
+  for (uint32_t k = 0; k < kTile / 16; ++k)
     ptx::umma_f16_a_tmem_if(issue, d, a_column(k), b_desc + uint64_t(k * 128u), kIdesc, k != 0 || accumulate ? 1u : 0u);
 }
 
