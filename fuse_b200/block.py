@@ -27,7 +27,8 @@ def _check(rc: int, what: str) -> None:
 
 
 def _within(bits: int, **numbers: int) -> None:
-    """Whole numbers that a record's signed field of `bits` holds (ctypes would cut off the rest without a word)."""
+    """Whole numbers that a record's signed field of `bits` holds (ctypes would cut off the rest without a word).
+    Names what does not; callers look first whether anything is that large, as the loop is a microsecond of a call's twenty."""
     for name, value in numbers.items():
         if not -(1 << (bits - 1)) <= value < 1 << (bits - 1):
             raise ValueError(f"{name}: {value} does not fit {bits} bits")
@@ -243,8 +244,9 @@ class Rotary:
     def record(self) -> N.RotarySpec:
         if self.scaling not in N.ROTARY_SCALINGS:
             raise ValueError(f"scaling: one of {sorted(N.ROTARY_SCALINGS)}, got {self.scaling!r}")
-        _within(32, rotary_dim=self.rotary_dim)
-        _within(64, original_context=self.original_context)
+        if abs(self.rotary_dim) >= 1 << 31 or abs(self.original_context) >= 1 << 63:
+            _within(32, rotary_dim=self.rotary_dim)
+            _within(64, original_context=self.original_context)
         return N.RotarySpec(self.theta, self.factor, self.low_freq_factor, self.high_freq_factor, self.beta_fast,
                             self.beta_slow, self.magnitude, self.original_context, self.rotary_dim,
                             N.ROTARY_SCALINGS[self.scaling], 1 if self.interleaved else 0)
@@ -312,7 +314,8 @@ def _rotary_arguments(q, k, spec, head_dim, seq_len, start, positions):
         raise ValueError(f"positions: expected contiguous int32 or int64 ({some.shape[0]},) on {some.device}")
     if seq_len is None:
         seq_len = max(1, some.shape[0])
-    _within(64, seq_len=seq_len, start=start)
+    if abs(seq_len) >= 1 << 63 or abs(start) >= 1 << 63:
+        _within(64, seq_len=seq_len, start=start)
     return spec.record(), seq_len
 
 
@@ -461,7 +464,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
     if window < 0 or sinks < 0 or (window and not causal):
         raise ValueError("window and sinks are not negative, and a window goes with causal attention")
     q_len, kv_len = q.shape[0] // batch if q_len is None else q_len, k.shape[0] // batch if kv_len is None else kv_len
-    _within(32, batch=batch, q_len=q_len, kv_len=kv_len, window=window, sinks=sinks)
+    if max(batch, q_len, kv_len, window, sinks) >= 1 << 31 or min(q_len, kv_len) < 0:
+        _within(32, batch=batch, q_len=q_len, kv_len=kv_len, window=window, sinks=sinks)
     shape = (batch, q_len, kv_len,
              q.shape[1] // head_dim, k.shape[1] // head_dim, head_dim, 1 if causal else 0, window, sinks,
              head_dim ** -0.5 if scale is None else scale, q_starts, q_lengths, kv_starts, kv_lengths)
