@@ -50,11 +50,13 @@ inline WaitContext make_wait(const DeviceInfo& info, uint32_t epoch, uint64_t bu
   return w;
 }
 
+// `most_smem`: the largest dynamic size that any launch of this kernel asks for.  The limit belongs to the kernel and not to
+// a launch: a thread that set it to its own smaller size between another's setting and launch would have that one refused.
 template <class Kernel, class... Args>
-cudaError_t launch_kernel(Kernel kernel, int grid, int threads, uint32_t dynamic_smem,
-                          bool cooperative, cudaStream_t stream, Args... args) {
+cudaError_t launch_kernel_sized(Kernel kernel, int grid, int threads, uint32_t dynamic_smem, uint32_t most_smem,
+                                bool cooperative, cudaStream_t stream, Args... args) {
   cudaError_t status =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(dynamic_smem));
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most_smem));
   if (status != cudaSuccess) return status;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(grid), 1, 1);
@@ -69,6 +71,12 @@ cudaError_t launch_kernel(Kernel kernel, int grid, int threads, uint32_t dynamic
   status = cudaLaunchKernelEx(&config, kernel, args...);
   if (status == cudaSuccess) count_launch();
   return status;
+}
+// A kernel whose launches all ask for the same size.
+template <class Kernel, class... Args>
+cudaError_t launch_kernel(Kernel kernel, int grid, int threads, uint32_t dynamic_smem,
+                          bool cooperative, cudaStream_t stream, Args... args) {
+  return launch_kernel_sized(kernel, grid, threads, dynamic_smem, dynamic_smem, cooperative, stream, args...);
 }
 
 inline bool aligned16(const void* p) {

@@ -522,9 +522,10 @@ cudaError_t rms_norm_backward(const fuse_b200_rms_norm_backward_params& p, cudaS
   a.wait = host::make_wait(info, 0, 0);
   if (grid > 0) {
     const int vec = (p.hidden + threads * 8 - 1) / (threads * 8);
-    const uint32_t shared = uint32_t(2 * 3 * 2 * p.hidden);
+    constexpr uint32_t kElementBytes = 2 * 3 * 2;  // of shared memory: two stages of three BF16 rows
     if (threads > 32) {
-      status = host::launch_kernel(rms_norm_backward_kernel, int(grid), threads, shared, false, stream, a);
+      status = host::launch_kernel_sized(rms_norm_backward_kernel, int(grid), threads, kElementBytes * uint32_t(p.hidden),
+                                         kElementBytes * uint32_t(kMaxHidden), false, stream, a);
     } else {
       if (vec == 1) rms_norm_backward_warp_kernel<1><<<grid, 128, 0, stream>>>(a);
       else rms_norm_backward_warp_kernel<2><<<grid, 128, 0, stream>>>(a);
