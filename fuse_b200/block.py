@@ -445,8 +445,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, head_dim: in
 
     The rows are `batch` sequences of q_len queries and kv_len keys (default: all rows, evenly), one behind the other.
     Shorter ones have their lengths in q_lengths / kv_lengths, others their first rows in q_starts / kv_starts
-    (int32 [batch] on the device; q_len and kv_len are then the longest).  Sequences may share keys (equal
-    kv_starts) only without gradients.  Queries are the last q_length positions of their sequence.  With `causal`,
+    (int32 [batch] on the device; q_len and kv_len are then the longest: what a length has beyond them is
+    cut off).  Sequences may share keys (equal kv_starts) only without gradients, and never queries.  Queries are the last q_length positions of their sequence.  With `causal`,
     `window` limits a query to the last `window` keys up to its own and the first `sinks` of the sequence.  Rows of
     no sequence are zeros in the result (with `out`: as they were).
     `out`: a tensor to write to, such as UlyssesProjections.attention_buffer() -- without gradients only, since a

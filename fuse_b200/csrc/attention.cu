@@ -40,7 +40,9 @@ int64_t query_blocks(const fuse_b200_attention_params& p) {
 
 // Splits over keys: when the query blocks do not fill the SMs, the number of splits whose waves of blocks
 // take the least time, in units of one key tile per block.  kFixed is what a block costs besides its tiles
-// (set-up, first loads, its partial result); a further split has to win by the joining kernel's cost.
+// (set-up, first loads, its partial result); a further split has to win by the joining kernel's cost.  From one block per SM on
+// nothing is weighed and nothing split; what that costs is the last wave: 144 blocks of 16384 keys (18 sequences of one token, 32 / 8
+// heads of 128) take 218 us, 160 of them 428.
 int32_t plan_splits(const fuse_b200_attention_params& p, int sm_count) {
   const int64_t blocks = query_blocks(p);
   int64_t keys = p.kv_len;
