@@ -315,7 +315,7 @@ class AttentionParams(C.Structure):
                 ("kv_starts", C.c_void_p), ("kv_lengths", C.c_void_p), ("batch", C.c_int32), ("q_len", C.c_int32),
                 ("kv_len", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
                 ("window", C.c_int32), ("sinks", C.c_int32), ("causal", C.c_uint8), ("scale", C.c_float),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("output_rest", C.c_void_p)]
 
 
 class AttentionBackwardParams(C.Structure):

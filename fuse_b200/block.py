@@ -371,12 +371,14 @@ def _partial(q, k, shape) -> bool:
     return any(t is not None for t in shape[10:]) or shape[0] * shape[1] != q.shape[0] or shape[0] * shape[2] != k.shape[0]
 
 
-def _attention_forward(q, k, v, shape, out, want_lse):
+def _attention_forward(q, k, v, shape, out, want_lse, rest=None):
     ragged = _partial(q, k, shape)
     if out is None:  # rows of no sequence are zeros here; the operator leaves them as they are
         out = (torch.zeros if ragged else torch.empty)(q.shape, dtype=BF16, device=q.device)
     p = _attention_record(q, k, v, shape)
     p.output, p.output_stride = out.data_ptr(), _stride(out)
+    if rest is not None:
+        p.output_rest = rest.data_ptr()
     lse = None
     if want_lse:
         lse = torch.empty((shape[3], q.shape[0]), dtype=torch.float32, device=q.device)
@@ -393,7 +395,7 @@ def _attention_forward(q, k, v, shape, out, want_lse):
     return out, lse
 
 
-def _attention_backward(do, q, k, v, out, lse, shape):
+def _attention_backward(do, q, k, v, out, rest, lse, shape):
     # one allocation (and, where rows may belong to no sequence, one clearing) for the three
     make = torch.zeros if _partial(q, k, shape) or not q.shape[0] else torch.empty
     nq, nk = q.shape[0] * q.shape[1], k.shape[0] * k.shape[1]
@@ -406,6 +408,7 @@ def _attention_backward(do, q, k, v, out, lse, shape):
     p = N.AttentionBackwardParams()
     p.forward = _attention_record(q, k, v, shape)
     p.forward.output, p.forward.output_stride, p.forward.lse = out.data_ptr(), _stride(out), lse.data_ptr()
+    p.forward.output_rest = rest.data_ptr()
     p.grad_output, p.grad_output_stride = do.data_ptr(), _stride(do)
     p.grad_q, p.grad_k, p.grad_v = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     p.grad_q_stride = p.grad_k_stride = p.grad_v_stride = -1
@@ -422,8 +425,10 @@ def _attention_backward(do, q, k, v, out, lse, shape):
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, shape, want_lse):
-        out, lse = _attention_forward(q, k, v, shape, None, want_lse)
-        ctx.save_for_backward(q, k, v, out, lse, *shape[10:])
+        # what rounding takes off the output, a byte an element: rowsum(do * out) would carry it into every gradient
+        rest = torch.empty(q.shape, dtype=torch.int8, device=q.device)
+        out, lse = _attention_forward(q, k, v, shape, None, want_lse, rest)
+        ctx.save_for_backward(q, k, v, out, rest, lse, *shape[10:])
         ctx.shape = shape[:10]
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -431,8 +436,8 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, _lse):
-        q, k, v, out, lse, *rows = ctx.saved_tensors
-        dq, dk, dv = _attention_backward(do, q, k, v, out, lse, (*ctx.shape, *rows))
+        q, k, v, out, rest, lse, *rows = ctx.saved_tensors
+        dq, dk, dv = _attention_backward(do, q, k, v, out, rest, lse, (*ctx.shape, *rows))
         return dq, dk, dv, None, None
 
 

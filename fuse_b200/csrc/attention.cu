@@ -105,6 +105,7 @@ attn::Args fill_args(const fuse_b200_attention_params& p) {
   a.scale = p.scale;
   a.scale_log2 = p.scale * attn::kLog2e;
   a.out = p.output;
+  a.rest = p.output_rest;
   a.lse = p.lse;
   a.splits = a.parts = 1;
   return a;
@@ -143,7 +144,7 @@ cudaError_t attention(const fuse_b200_attention_params& p, const fuse_b200_optio
   if (p.batch == 0 || p.q_len == 0 || p.q_rows == 0) return cudaSuccess;
   if (!aligned_rows(p.q, q_stride, q_width) || !aligned_rows(p.output, out_stride, q_width) ||
       (p.kv_rows > 0 && (!aligned_rows(p.k, k_stride, kv_width) || !aligned_rows(p.v, v_stride, kv_width))) ||
-      (p.lse != nullptr && !host::aligned4(p.lse)))
+      (p.output_rest != nullptr && !host::aligned16(p.output_rest)) || (p.lse != nullptr && !host::aligned4(p.lse)))
     return cudaErrorInvalidValue;
   DeviceInfo info;
   if ((status = launch::check_device(&info)) != cudaSuccess) return status;
@@ -277,7 +278,7 @@ cudaError_t attention_backward(const fuse_b200_attention_backward_params& g, con
   if (p.q_rows == 0) return cudaErrorInvalidValue;  // key gradients of no query: the caller's zeros
   if (!aligned_rows(p.q, q_stride, q_width) || !aligned_rows(p.output, b.o_stride, q_width) ||
       !aligned_rows(g.grad_output, b.do_stride, q_width) || !aligned_rows(g.grad_q, b.dq_stride, q_width) ||
-      !host::aligned4(p.lse) ||
+      !host::aligned4(p.lse) || (p.output_rest != nullptr && !host::aligned16(p.output_rest)) ||
       (p.kv_rows > 0 && (!aligned_rows(p.k, k_stride, kv_width) || !aligned_rows(p.v, v_stride, kv_width) ||
                          !aligned_rows(g.grad_k, b.dk_stride, kv_width) || !aligned_rows(g.grad_v, b.dv_stride, kv_width))) ||
       g.workspace == nullptr || reinterpret_cast<uintptr_t>(g.workspace) % 256 != 0 || g.workspace_bytes < delta_bytes(p))

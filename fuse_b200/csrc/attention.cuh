@@ -52,6 +52,7 @@ struct Args {
   int32_t causal, window, sinks;
   float scale, scale_log2;
   uint16_t* out;
+  int8_t* rest;  // [q_rows][q_heads * head_dim] what rounding takes off out, or nullptr
   int64_t out_stride;
   float* lse;  // [q_heads][q_rows] or nullptr
   // split over keys: partial results per (part, batch, token, head), joined by a second kernel
@@ -265,6 +266,19 @@ struct Columns {
   uint32_t base;
   __device__ __forceinline__ uint32_t operator()(uint32_t k) const { return base + k * 8u; }
 };
+
+// What rounding to BF16 takes off an FP32 value, as a byte: the difference of the bit patterns in units of 2^8 (half a step of BF16 is
+// 2^15), so that value and byte together keep 16 bits of the fraction.  Infinities and NaN stay what they are.
+__device__ __forceinline__ int32_t rounded_off(float v, uint32_t bf16_bits) {
+  const int32_t difference = int32_t(__float_as_uint(v) - (bf16_bits << 16));
+  return max(min((difference + 128) >> 8, 127), -128);
+}
+__device__ __forceinline__ float with_rest(uint32_t bf16_bits, int32_t rest) {
+  return __uint_as_float((bf16_bits << 16) + uint32_t(rest * 256));
+}
+__device__ __forceinline__ uint32_t rest_of_pair(uint32_t pair, float lo, float hi) {  // two bytes
+  return (uint32_t(rounded_off(lo, pair & 0xffffu)) & 0xffu) | ((uint32_t(rounded_off(hi, pair >> 16)) & 0xffu) << 8);
+}
 
 template <int kDim>
 struct ForwardLayout {
@@ -581,12 +595,20 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int i = 0; i < 8; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           } else {
             uint4* to = reinterpret_cast<uint4*>(a.out + out_row * a.out_stride + int64_t(head) * kDim + c);
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              to[i] = make_uint4(pack_bf16(as_float(o[8 * i]), as_float(o[8 * i + 1])),
-                                 pack_bf16(as_float(o[8 * i + 2]), as_float(o[8 * i + 3])),
-                                 pack_bf16(as_float(o[8 * i + 4]), as_float(o[8 * i + 5])),
-                                 pack_bf16(as_float(o[8 * i + 6]), as_float(o[8 * i + 7])));
+            for (int i = 0; i < 16; ++i) w[i] = pack_bf16(as_float(o[2 * i]), as_float(o[2 * i + 1]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            if (a.rest != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = rest_of_pair(w[i], as_float(o[2 * i]), as_float(o[2 * i + 1]));
+              uint4* rest = reinterpret_cast<uint4*>(a.rest + (out_row * a.q_heads + head) * kDim + c);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                rest[i] = make_uint4(w[8 * i] | (w[8 * i + 1] << 16), w[8 * i + 2] | (w[8 * i + 3] << 16),
+                                     w[8 * i + 4] | (w[8 * i + 5] << 16), w[8 * i + 6] | (w[8 * i + 7] << 16));
+            }
           }
         }
       }
@@ -637,8 +659,14 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
   const int64_t row = int64_t(seq.q0) + token;
   uint16_t* to = a.out + row * a.out_stride + int64_t(head) * kDim + lane * kEach;
+  int8_t* rest = a.rest + (row * a.q_heads + head) * kDim + lane * kEach;
 #pragma unroll
-  for (int i = 0; i < kEach; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack_bf16(acc[i] * inverse, acc[i + 1] * inverse);
+  for (int i = 0; i < kEach; i += 2) {
+    const float x = acc[i] * inverse, y = acc[i + 1] * inverse;
+    const uint32_t w = pack_bf16(x, y);
+    *reinterpret_cast<uint32_t*>(to + i) = w;
+    if (a.rest != nullptr) *reinterpret_cast<uint16_t*>(rest + i) = uint16_t(rest_of_pair(w, x, y));
+  }
   if (lane == 0 && a.lse != nullptr)
     a.lse[int64_t(head) * a.q_rows + row] = sum != 0.0f ? m + logf(sum) : -INFINITY;
 }

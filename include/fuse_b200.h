@@ -663,6 +663,9 @@ FUSE_API int fuse_b200_launch_rotary(const fuse_b200_rotary_params* params, fuse
  * infinity in a key or value of the sequence itself may reach queries that do not see it.
  *
  * `lse` (may be NULL): FP32 [q_heads][q_rows], log of the sum of exp(scale q k) -- what the backward needs.
+ * `output_rest` (may be NULL, 16-byte aligned): int8 [q_rows][q_heads * head_dim], what rounding took off output: the FP32 value's bits are
+ * (output << 16) + (output_rest << 8) within 2^8.  With it the backward's rowsum(grad_output * output) is right to 2^-16 of its terms;
+ * without it that sum carries output's rounding into every gradient, which shows where a row's weight lies on few keys.
  * `output` must not overlap an input.  `workspace` (256-byte aligned, fuse_b200_attention_workspace_size; may be 0 bytes) holds partial results when
  * the keys are split because the queries alone would leave SMs idle; two launches that may run at the same
  * time need two. */
@@ -682,13 +685,14 @@ typedef struct fuse_b200_attention_params {
   float scale; /* > 0 */
   void* workspace;
   size_t workspace_bytes;
+  int8_t* output_rest;
 } fuse_b200_attention_params;
 FUSE_API int fuse_b200_attention_workspace_size(const fuse_b200_attention_params* params, size_t* bytes);
 FUSE_API int fuse_b200_launch_attention(const fuse_b200_attention_params* params, const fuse_b200_options* options,
                                         fuse_stream stream);
 
-/* Gradients of the above.  `forward`: the forward's record, with its output and lse as inputs (its workspace is not
- * used).  grad_q like q, grad_k and grad_v like k: rows of the sequences are written, others left as they
+/* Gradients of the above.  `forward`: the forward's record, with its output, output_rest and lse as inputs (its workspace
+ * is not used).  grad_q like q, grad_k and grad_v like k: rows of the sequences are written, others left as they
  * were; none of them may overlap an input.  q_rows must not be 0 where kv_rows is not, and sequences must not share
  * rows (the forward alone may read the same keys for several).  No atomics: the same inputs give the same bits.
  * workspace: 256-byte aligned, fuse_b200_attention_backward_workspace_size bytes. */

@@ -4,7 +4,8 @@ import random
 import pytest
 import torch
 
-from fuse_b200 import block
+from fuse_b200 import api, block
+from tests.test_block_host import INVALID, PTR, attention_backward_params, attention_params
 
 
 def test_overlap_of_row_views_against_enumeration():
@@ -39,3 +40,11 @@ def test_numbers_that_a_record_would_cut_off():
         block.Rotary((1 << 32) + 64).record()
     with pytest.raises(ValueError, match="original_context"):
         block.Rotary(64, scaling="yarn", factor=2.0, original_context=(1 << 64) + 8192).frequencies()
+
+
+def test_attention_refuses_an_unaligned_rest():
+    p = attention_params(output_rest=PTR + 8)
+    assert api.launch_attention(p) == INVALID
+    assert api.launch_attention_backward(attention_backward_params(output_rest=PTR + 8)) == INVALID
+    if not torch.cuda.is_available():  # an aligned one passes the checks and meets the missing device
+        assert api.launch_attention(attention_params(output_rest=PTR + 16)) not in (0, INVALID)
