@@ -26,6 +26,17 @@ def _check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} -> cudaError {rc}")
 
 
+def _refused(rc: int, what: str, tensors: dict, **limits: bool) -> None:
+    """Raises for a launch that gave `rc`, with what of its arguments explains it: rows that are not where vectors can be
+    read, and the limits that are not kept (description=whether it is)."""
+    reasons = [f"{name} is not on a 16-byte boundary" for name, t in tensors.items() if t is not None and t.numel() and t.data_ptr() % 16]
+    reasons += [f"{name}'s rows are {t.stride(0)} elements apart, not a multiple of 8 from {t.shape[1]} on"
+                for name, t in tensors.items()
+                if t is not None and t.dim() == 2 and t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])]
+    reasons += [name for name, kept in limits.items() if not kept]
+    raise RuntimeError(f"{what} -> cudaError {rc}" + (": " + "; ".join(reasons) if reasons else ""))
+
+
 def _within(bits: int, **numbers: int) -> None:
     """Whole numbers that a record's signed field of `bits` holds (ctypes would cut off the rest without a word).
     Names what does not; callers look first whether anything is that large, as the loop is a microsecond of a call's twenty."""
@@ -148,7 +159,10 @@ def _norm_forward(x, gamma, residual, eps, output: bool, mxfp8: bool):
         p.quantized.data_bytes, p.quantized.scale_bytes = data.numel(), scales.numel()
     if rows:
         with _On(x) as stream:
-            _check(N.lib().fuse_b200_launch_rms_norm(C.byref(p), stream), "launch_rms_norm")
+            rc = N.lib().fuse_b200_launch_rms_norm(C.byref(p), stream)
+        if rc:
+            _refused(rc, "launch_rms_norm", dict(x=x, gamma=gamma, residual=residual), **{
+                "hidden is a multiple of 8, at most 16384": hidden % 8 == 0 and hidden <= 16384, "eps is at least 1e-30": eps >= 1e-30})
     return y, h, data, scales
 
 
@@ -274,7 +288,13 @@ def _rotary_launch(q, k, qo, ko, spec, head_dim, seq_len, start, positions, adjo
     p.position_start, p.rows, p.seq_len = start, some.shape[0], seq_len
     p.head_dim, p.spec, p.adjoint = head_dim, spec, adjoint
     with _On(some) as stream:
-        _check(N.lib().fuse_b200_launch_rotary(C.byref(p), stream), "launch_rotary")
+        rc = N.lib().fuse_b200_launch_rotary(C.byref(p), stream)
+    if rc:
+        raise RuntimeError(f"launch_rotary -> cudaError {rc}" + (
+            f": rotary_dim is even and within 2 .. head_dim, at most 256, got {spec.rotary_dim} of {head_dim}"
+            if not 2 <= spec.rotary_dim <= min(head_dim, 256) or spec.rotary_dim % 2 else
+            ": the specification's scaling has no such parameters" if N.lib().fuse_b200_rotary_frequencies(
+                C.byref(spec), (C.c_double * 128)(), C.byref(C.c_double())) else ""))
 
 
 class _Rotary(torch.autograd.Function):
@@ -387,11 +407,18 @@ def _attention_forward(q, k, v, shape, out, want_lse, rest=None):
         p.lse = lse.data_ptr()
     with _On(q) as stream:
         size = C.c_size_t()
-        _check(N.lib().fuse_b200_attention_workspace_size(C.byref(p), C.byref(size)), "attention_workspace_size")
-        if size.value:
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device)
-            p.workspace, p.workspace_bytes = workspace.data_ptr(), size.value
-        _check(N.lib().fuse_b200_launch_attention(C.byref(p), None, stream), "launch_attention")
+        rc = N.lib().fuse_b200_attention_workspace_size(C.byref(p), C.byref(size))
+        if not rc:
+            if size.value:
+                workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device)
+                p.workspace, p.workspace_bytes = workspace.data_ptr(), size.value
+            rc = N.lib().fuse_b200_launch_attention(C.byref(p), None, stream)
+    if rc:
+        _refused(rc, "launch_attention", dict(q=q, k=k, v=v, out=out), **{
+            "head_dim is 64 or 128": p.head_dim in (64, 128), "scale is positive and finite": 0.0 < p.scale < float("inf"),
+            "q_len and kv_len are not negative": p.q_len >= 0 and p.kv_len >= 0,
+            "batch * q_len rows are in q": shape[10] is not None or p.batch * p.q_len <= p.q_rows,
+            "batch * kv_len rows are in k and v": shape[12] is not None or p.batch * p.kv_len <= p.kv_rows})
     return out, lse
 
 

@@ -141,3 +141,24 @@ def test_gradient_beside_the_mxfp8_form(rows, hidden):
     assert all(torch.equal(a, b) for a, b in zip(*results))
     h2, data, scales = block.rms_norm_mxfp8(x, gamma, residual)
     assert torch.equal(h2, results[1][1]) and torch.equal(data, packed[0]) and torch.equal(scales, packed[1])
+
+
+# ---- a refusal names its reason
+def test_refusals_name_their_reason():
+    x, gamma, q = randn(8, 512), randn(512), randn(8, 128)
+    odd = randn(8, 136)[:, :128].as_strided((7, 128), (132, 1))
+    for call, words in (
+            (lambda: block.rms_norm(x[:, 4:260], gamma[:256]), "x is not on a 16-byte boundary"),
+            (lambda: block.rms_norm(x[:, :256], gamma[4:260]), "gamma is not on a 16-byte boundary"),
+            (lambda: block.rms_norm(x[:, :252], gamma[:252]), "hidden is a multiple of 8"),
+            (lambda: block.rms_norm(x, gamma, eps=0.0), "eps"),
+            (lambda: block.rotary(q, None, block.Rotary(128), head_dim=64), "rotary_dim"),
+            (lambda: block.rotary(q, None, block.Rotary(64, scaling="yarn", factor=2.0), head_dim=64), "scaling"),
+            (lambda: block.attention(q, q, q, head_dim=32), "head_dim is 64 or 128"),
+            (lambda: block.attention(q, q, q, head_dim=64, scale=0.0), "scale"),
+            (lambda: block.attention(q, q, q, head_dim=64, q_len=9), "rows are in q"),
+            (lambda: block.attention(q, q, q, head_dim=64, kv_len=9), "rows are in k"),
+            (lambda: block.attention(q, q, q, head_dim=64, q_len=-1), "not negative"),
+            (lambda: block.attention(odd, q[:7], q[:7], head_dim=64), "q's rows are 132 elements apart")):
+        with pytest.raises(RuntimeError, match=words):
+            call()
